@@ -11,7 +11,9 @@
 #include "comm/nccl_utils.h"
 #include "elementwise/fo_elementwise.h"
 #include "flags/fo_wait.h"
+#include "moe/fo_moe.h"
 #include "norm/fo_norm.h"
+#include "norm/fo_norm_block.h"
 #include "runtime/baseline_impl.h"
 #include "runtime/fused_common.h"
 #include "runtime/loopback.h"
@@ -114,6 +116,242 @@ void add_rmsnorm(at::Tensor X, at::Tensor T, at::Tensor H, at::Tensor RX, at::Te
                                         static_cast<float>(eps), bf, sm_count_of_current_device(),
                                         c10::cuda::getCurrentCUDAStream().stream()),
                  "add_rmsnorm");
+}
+
+// What the ops that return new tensors read from: contiguous and 16-byte aligned, copied if it is not.
+at::Tensor dense(const at::Tensor& t) {
+  at::Tensor d = t.contiguous();
+  return aligned16(d) ? d : d.clone();
+}
+
+void check_16bit(const at::Tensor& t, const char* name) {
+  FO_CHECK(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf), name,
+           " must be a bfloat16 or float16 CUDA tensor");
+}
+
+bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+
+// The operands of rmsnorm_add_rmsnorm and of its backward pass, checked.
+struct NormBlockOperands {
+  at::Tensor X, T, PW, W, G;
+  fo::NormBlock p;
+};
+NormBlockOperands norm_block_operands(const at::Tensor& X, const at::Tensor& T, const at::Tensor& PW, const at::Tensor& W,
+                                      const c10::optional<at::Tensor>& G, double alpha, double eps) {
+  check_16bit(X, "X");
+  FO_CHECK(X.dim() == 2 && T.sizes() == X.sizes(), "X and T must be [rows, dim]");
+  const int64_t rows = X.size(0), dim = X.size(1);
+  FO_CHECK(dim >= 8 && dim % 8 == 0 && dim <= 16384, "dim must be a multiple of 8 from 8 to 16384 (", dim, ")");
+  FO_CHECK(rows <= INT32_MAX, "too many rows");
+  FO_CHECK(PW.dim() == 1 && PW.size(0) == dim && W.dim() == 1 && W.size(0) == dim, "PW and W must be [dim]");
+  int64_t lines = 1;
+  if (given(G)) {
+    FO_CHECK((G->dim() == 1 || G->dim() == 2) && G->size(-1) == dim, "G must be [dim] or [lines, dim]");
+    if (G->dim() == 2) lines = G->size(0);
+    FO_CHECK(rows == 0 || (lines >= 1 && rows % lines == 0), "rows must be a multiple of G's lines (", rows, ", ", lines, ")");
+    fo::check_device(*G, X, "G");
+    FO_CHECK(G->scalar_type() == X.scalar_type(), "X, T, PW, W and G must share a dtype");
+  }
+  for (const at::Tensor& t : {T, PW, W}) {
+    fo::check_device(t, X, "an operand");
+    FO_CHECK(t.scalar_type() == X.scalar_type(), "X, T, PW, W and G must share a dtype");
+  }
+  NormBlockOperands o{dense(X), dense(T), dense(PW), dense(W), given(G) ? dense(*G) : at::Tensor(), {}};
+  o.p.X = o.X.data_ptr();
+  o.p.T = o.T.data_ptr();
+  o.p.PW = o.PW.data_ptr();
+  o.p.W = o.W.data_ptr();
+  o.p.G = o.G.defined() ? o.G.data_ptr() : nullptr;
+  o.p.rows = static_cast<int>(rows);
+  o.p.dim = static_cast<int>(dim);
+  o.p.lines = static_cast<int>(lines);
+  o.p.alpha = static_cast<float>(alpha);
+  o.p.eps = static_cast<float>(eps);
+  o.p.bf16 = X.scalar_type() == at::kBFloat16;
+  return o;
+}
+
+// (H, Y, stats): u = rmsnorm(T) * PW, H = alpha * X + G * u, Y = rmsnorm(H) * W; stats [rows, 2] fp32 (1 / rms of T and of H),
+// what the backward pass needs, if asked for, else empty.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_add_rmsnorm(at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
+                                                                    c10::optional<at::Tensor> G, double alpha, double eps,
+                                                                    bool with_stats) {
+  check_16bit(X, "X");
+  c10::cuda::CUDAGuard guard(X.device());
+  const NormBlockOperands o = norm_block_operands(X, T, PW, W, G, alpha, eps);
+  at::Tensor H = at::empty(X.sizes(), o.X.options()), Y = at::empty(X.sizes(), o.X.options());
+  at::Tensor stats = at::empty({with_stats ? X.size(0) : 0, 2}, o.X.options().dtype(at::kFloat));
+  if (o.p.rows > 0) {
+    fo::cuda_check(fo::norm_block_launch(o.p, H.data_ptr(), Y.data_ptr(), with_stats ? stats.data_ptr<float>() : nullptr,
+                                         sm_count_of_current_device(), c10::cuda::getCurrentCUDAStream().stream()),
+                   "rmsnorm_add_rmsnorm");
+  }
+  return {H, Y, stats};
+}
+
+// Gradients of X, T, PW, W and G (empty without G) from those of H and Y (either may be absent: zero).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm_add_rmsnorm_backward(
+    c10::optional<at::Tensor> GH, c10::optional<at::Tensor> GY, at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
+    c10::optional<at::Tensor> G, at::Tensor stats, double alpha) {
+  check_16bit(X, "X");
+  c10::cuda::CUDAGuard guard(X.device());
+  const NormBlockOperands o = norm_block_operands(X, T, PW, W, G, alpha, 0.);
+  at::Tensor gh, gy;
+  for (const auto& [from, to] : {std::pair{&GH, &gh}, std::pair{&GY, &gy}}) {
+    if (!given(*from)) continue;
+    const at::Tensor& g = **from;
+    FO_CHECK(g.sizes() == X.sizes() && g.scalar_type() == X.scalar_type(), "GH and GY must be like X");
+    fo::check_device(g, X, "a gradient");
+    *to = dense(g);
+  }
+  FO_CHECK(stats.is_cuda() && stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.dim() == 2 &&
+               stats.size(0) == X.size(0) && stats.size(1) == 2,
+           "stats must be what the forward pass returned");
+  fo::check_device(stats, X, "stats");
+  const auto options = o.X.options();
+  at::Tensor DX = at::empty(X.sizes(), options), DT = at::empty(X.sizes(), options);
+  const bool none = o.p.rows == 0;
+  at::Tensor DPW = none ? at::zeros_like(o.PW) : at::empty_like(o.PW), DW = none ? at::zeros_like(o.W) : at::empty_like(o.W);
+  at::Tensor DG = !o.G.defined() ? at::empty({0}, options) : (none ? at::zeros_like(o.G) : at::empty_like(o.G));
+  if (!none) {
+    const fo::NormBlockPlan plan = fo::norm_block_plan(o.p, sm_count_of_current_device());
+    at::Tensor workspace = at::empty({static_cast<int64_t>(plan.workspace)}, options.dtype(at::kFloat));
+    fo::cuda_check(fo::norm_block_backward_launch(o.p, stats.data_ptr<float>(), gh.defined() ? gh.data_ptr() : nullptr,
+                                                  gy.defined() ? gy.data_ptr() : nullptr, DX.data_ptr(), DT.data_ptr(),
+                                                  DPW.data_ptr(), DW.data_ptr(), DG.data_ptr(), workspace.data_ptr<float>(),
+                                                  plan, c10::cuda::getCurrentCUDAStream().stream()),
+                   "rmsnorm_add_rmsnorm_backward");
+  }
+  return {DX, DT, DPW, DW, DG};
+}
+
+// (slot [tokens, top_k], source [tokens * top_k], offsets [experts + 1]) of the experts `ids` [tokens, top_k] chosen for each token.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_sort(at::Tensor ids, int64_t experts) {
+  FO_CHECK(ids.is_cuda() && ids.dim() == 2 && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
+           "ids must be an int32 or int64 CUDA tensor [tokens, top_k]");
+  FO_CHECK(experts >= 1 && experts <= fo::kMaxExperts, "experts must be from 1 to ", fo::kMaxExperts, " (", experts, ")");
+  FO_CHECK(ids.size(1) >= 1 && ids.size(1) <= fo::kMaxTopK, "top_k must be from 1 to ", fo::kMaxTopK, " (", ids.size(1), ")");
+  FO_CHECK(ids.numel() <= INT32_MAX, "too many choices");
+  c10::cuda::CUDAGuard guard(ids.device());
+  const at::Tensor c = ids.contiguous();
+  const auto options = c.options().dtype(at::kInt);
+  at::Tensor slot = at::empty(ids.sizes(), options), source = at::empty({ids.numel()}, options);
+  at::Tensor offsets = at::empty({experts + 1}, options);
+  fo::cuda_check(fo::moe_sort_launch(c.data_ptr(), c.scalar_type() == at::kLong, c.numel(), static_cast<int>(experts),
+                                     slot.data_ptr<int>(), source.data_ptr<int>(), offsets.data_ptr<int>(),
+                                     c10::cuda::getCurrentCUDAStream().stream()),
+                 "moe_sort");
+  return {slot, source, offsets};
+}
+
+// Shape of a call over rows of `like`, with the order's tensors checked.
+fo::MoeShape moe_shape(const at::Tensor& like, int64_t dim, const at::Tensor& slot, const at::Tensor* offsets) {
+  FO_CHECK(slot.is_cuda() && slot.is_contiguous() && slot.scalar_type() == at::kInt && slot.dim() == 2,
+           "slot must be a contiguous int32 CUDA tensor [tokens, top_k]");
+  fo::check_device(slot, like, "slot");
+  FO_CHECK(slot.size(1) >= 1 && slot.size(1) <= fo::kMaxTopK && slot.numel() <= INT32_MAX, "top_k must be from 1 to ", fo::kMaxTopK);
+  FO_CHECK(dim >= 8 && dim % 8 == 0 && dim <= INT32_MAX, "dim must be a multiple of 8 (", dim, ")");
+  fo::MoeShape s{static_cast<int>(slot.size(0)), static_cast<int>(slot.size(1)), static_cast<int>(dim), 1,
+                 like.scalar_type() == at::kBFloat16};
+  if (offsets != nullptr) {
+    FO_CHECK(offsets->is_cuda() && offsets->is_contiguous() && offsets->scalar_type() == at::kInt && offsets->dim() == 1 &&
+                 offsets->numel() >= 2 && offsets->numel() <= fo::kMaxExperts + 1,
+             "offsets must be a contiguous int32 CUDA tensor [experts + 1]");
+    fo::check_device(*offsets, like, "offsets");
+    s.experts = static_cast<int>(offsets->numel()) - 1;
+  }
+  return s;
+}
+
+// The router's weights, contiguous; none: undefined.
+at::Tensor moe_weights(const c10::optional<at::Tensor>& weights, const at::Tensor& like, const at::Tensor& slot) {
+  if (!given(weights)) return {};
+  FO_CHECK(weights->sizes() == slot.sizes() && (weights->scalar_type() == at::kFloat || weights->scalar_type() == like.scalar_type()),
+           "weights must be [tokens, top_k], float32 or of the rows' dtype");
+  fo::check_device(*weights, like, "weights");
+  return weights->contiguous();
+}
+
+fo::MoeWeights weights_arg(const at::Tensor& w) {
+  return w.defined() ? fo::MoeWeights{w.data_ptr(), w.scalar_type() == at::kFloat} : fo::MoeWeights{nullptr, false};
+}
+
+// R [tokens * top_k, dim]: R[slot[t, k]] = X[t], the rows behind the last expert's zero.
+at::Tensor moe_dispatch(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
+  check_16bit(X, "X");
+  FO_CHECK(X.dim() == 2 && slot.dim() == 2 && X.size(0) == slot.size(0), "X must be [tokens, dim] and slot [tokens, top_k]");
+  c10::cuda::CUDAGuard guard(X.device());
+  const fo::MoeShape s = moe_shape(X, X.size(1), slot, &offsets);
+  const at::Tensor x = dense(X);
+  at::Tensor R = at::empty({slot.numel(), X.size(1)}, x.options());
+  if (s.tokens > 0) {
+    fo::cuda_check(fo::moe_dispatch_launch(s, x.data_ptr(), slot.data_ptr<int>(), offsets.data_ptr<int>(), R.data_ptr(),
+                                           c10::cuda::getCurrentCUDAStream().stream()),
+                   "moe_dispatch");
+  }
+  return R;
+}
+
+// O [tokens, dim]: the sum over k of weights[t, k] * R[slot[t, k]] (no weights: 1).
+at::Tensor moe_combine(at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot) {
+  check_16bit(R, "R");
+  FO_CHECK(R.dim() == 2 && R.size(0) == slot.numel(), "R must be [tokens * top_k, dim] and slot [tokens, top_k]");
+  c10::cuda::CUDAGuard guard(R.device());
+  const fo::MoeShape s = moe_shape(R, R.size(1), slot, nullptr);
+  const at::Tensor r = dense(R), w = moe_weights(weights, R, slot);
+  at::Tensor O = at::empty({slot.size(0), R.size(1)}, r.options());
+  if (s.tokens > 0) {
+    fo::cuda_check(fo::moe_combine_launch(s, r.data_ptr(), weights_arg(w), slot.data_ptr<int>(), O.data_ptr(),
+                                          c10::cuda::getCurrentCUDAStream().stream()),
+                   "moe_combine");
+  }
+  return O;
+}
+
+// (gradient of R, gradient of weights) from that of O; one that is not asked for comes back empty.
+std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::optional<at::Tensor> R,
+                                                        c10::optional<at::Tensor> weights, at::Tensor slot,
+                                                        at::Tensor offsets, bool for_rows, bool for_weights) {
+  check_16bit(GO, "GO");
+  FO_CHECK(GO.dim() == 2 && slot.dim() == 2 && GO.size(0) == slot.size(0), "GO must be [tokens, dim] and slot [tokens, top_k]");
+  FO_CHECK(for_rows || for_weights, "no gradient is asked for");
+  c10::cuda::CUDAGuard guard(GO.device());
+  const fo::MoeShape s = moe_shape(GO, GO.size(1), slot, &offsets);
+  const at::Tensor go = dense(GO), w = moe_weights(weights, GO, slot);
+  at::Tensor r, DR, DW;
+  if (for_weights) {
+    FO_CHECK(w.defined() && given(R), "the weights' gradient needs R and weights");
+    FO_CHECK(R->dim() == 2 && R->size(0) == slot.numel() && R->size(1) == GO.size(1) && R->scalar_type() == GO.scalar_type(),
+             "R must be [tokens * top_k, dim] of GO's dtype");
+    fo::check_device(*R, GO, "R");
+    r = dense(*R);
+  }
+  DR = at::empty({for_rows ? slot.numel() : 0, GO.size(1)}, go.options());
+  DW = for_weights ? at::empty(slot.sizes(), w.options()) : at::empty({0}, go.options());
+  if (s.tokens > 0) {
+    fo::cuda_check(fo::moe_combine_backward_launch(s, go.data_ptr(), r.defined() ? r.data_ptr() : nullptr, weights_arg(w),
+                                                   slot.data_ptr<int>(), offsets.data_ptr<int>(),
+                                                   for_rows ? DR.data_ptr() : nullptr, for_weights ? DW.data_ptr() : nullptr,
+                                                   c10::cuda::getCurrentCUDAStream().stream()),
+                   "moe_combine_backward");
+  }
+  return {DR, DW};
+}
+
+// (Q int8, S fp32 [rows]) of X [rows, dim].
+std::tuple<at::Tensor, at::Tensor> quantize_rows(at::Tensor X) {
+  check_16bit(X, "X");
+  FO_CHECK(X.dim() == 2 && X.size(0) <= INT32_MAX, "X must be [rows, dim]");
+  FO_CHECK(X.size(1) >= 8 && X.size(1) % 8 == 0 && X.size(1) <= fo::kMaxQuantizeDim, "dim must be a multiple of 8 from 8 to ",
+           fo::kMaxQuantizeDim, " (", X.size(1), ")");
+  c10::cuda::CUDAGuard guard(X.device());
+  const at::Tensor x = dense(X);
+  at::Tensor Q = at::empty(X.sizes(), x.options().dtype(at::kChar)), S = at::empty({X.size(0)}, x.options().dtype(at::kFloat));
+  fo::cuda_check(fo::quantize_rows_launch(x.data_ptr(), Q.data_ptr(), S.data_ptr<float>(), static_cast<int>(X.size(0)),
+                                          static_cast<int>(X.size(1)), x.scalar_type() == at::kBFloat16,
+                                          c10::cuda::getCurrentCUDAStream().stream()),
+                 "quantize_rows");
+  return {Q, S};
 }
 
 // Rotary embedding, in place, of the first `heads` heads of every row of QKV [tokens, row_elems].
@@ -268,6 +506,8 @@ TORCH_LIBRARY(flashoverlap_class, m) {
       .def("gemm_reducescatter_add_rmsnorm_fused", &OverlapImpl::GemmReduceScatterAddRmsNormFused)
       .def("gemm_add", &OverlapImpl::GemmAdd)
       .def("gemm_swiglu", &OverlapImpl::GemmSwiGLU)
+      .def("gemm_i8", &OverlapImpl::GemmI8)
+      .def("linear_i8", &OverlapImpl::LinearI8)
       .def("set_option", &OverlapImpl::SetOption)
       .def("get_option", &OverlapImpl::GetOption)
       .def("symm_empty", &OverlapImpl::SymmEmpty)
@@ -290,6 +530,13 @@ TORCH_LIBRARY(flashoverlap_op, m) {
   m.def("add_rmsnorm", &add_rmsnorm);
   m.def("rope_", &rope_);
   m.def("swiglu", &swiglu);
+  m.def("rmsnorm_add_rmsnorm", &rmsnorm_add_rmsnorm);
+  m.def("rmsnorm_add_rmsnorm_backward", &rmsnorm_add_rmsnorm_backward);
+  m.def("moe_sort", &moe_sort);
+  m.def("moe_dispatch", &moe_dispatch);
+  m.def("moe_combine", &moe_combine);
+  m.def("moe_combine_backward", &moe_combine_backward);
+  m.def("quantize_rows", &quantize_rows);
   m.def("reorder", &reorder);
   m.def("unreorder", &unreorder);
   m.def("wait_flag", &wait_flag);

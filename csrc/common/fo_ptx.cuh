@@ -231,6 +231,28 @@ FO_DEVICE void tma_load_2d_pair(void* smem_dst, const CUtensorMap* m, uint64_t* 
       : "memory");
 }
 
+// The 3-D forms of the two loads above.
+FO_DEVICE void tma_load_3d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int32_t c0, int32_t c1, int32_t c2,
+                           uint64_t l2_hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      :
+      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
+        "l"(l2_hint)
+      : "memory");
+}
+FO_DEVICE void tma_load_3d_pair(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int32_t c0, int32_t c1, int32_t c2,
+                                uint64_t l2_hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      :
+      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar) & kPeerBitMask), "r"(c0), "r"(c1),
+        "r"(c2), "l"(l2_hint)
+      : "memory");
+}
+
 // 2-D tiled store shared -> global (local or peer memory), tracked by this thread's bulk
 // async-group.  The store coordinate x * elem_size must be a multiple of 16 B and neither
 // coordinate may be negative.
@@ -373,6 +395,41 @@ FO_DEVICE void umma_f16_ss_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_
       : "memory");
 }
 
+// Instruction descriptor for tcgen05.mma.kind::i8: A, B both K-major signed 8-bit integers, 32-bit integer accumulate.
+FO_DEVICE constexpr uint32_t make_idesc_s8(int umma_m, int umma_n) {
+  uint32_t d = 0;
+  d |= 2u << 4;   // D format: S32
+  d |= 1u << 7;   // A format: signed
+  d |= 1u << 10;  // B format: signed
+  d |= static_cast<uint32_t>(umma_n >> 3) << 17;
+  d |= static_cast<uint32_t>(umma_m >> 4) << 24;
+  return d;
+}
+
+// The 8-bit integer forms of the two products above: 32 elements of K (32 bytes) an instruction.
+FO_DEVICE void umma_s8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+FO_DEVICE void umma_s8_ss_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive (once the pair's MMAs issued so far have completed) on the barrier at this offset in
 // every CTA of the cluster selected by `cta_mask`.  This multicast is a barrier signal, not a
 // data load.
@@ -415,6 +472,12 @@ FO_DEVICE void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+FO_DEVICE void tmem_ld_32x32b_x4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
 }
 FO_DEVICE void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 

@@ -3,6 +3,7 @@
 #include <cstdint>
 
 #include "../common/fo_pack16.cuh"
+#include "../common/fo_ptx.cuh"
 
 namespace fo {
 
@@ -92,7 +93,99 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// Bound by memory: 3 bytes an element.  A CTA takes a row, which stays in registers between the maximum and the rounding.
+constexpr int kQuantizeThreads = 512;
+
+template <bool BF16, int VPT>
+__global__ void __launch_bounds__(kQuantizeThreads)
+    quantize_rows_kernel(const uint16_t* __restrict__ X, int8_t* __restrict__ Q, float* __restrict__ S, int dim) {
+  __shared__ float red[kQuantizeThreads / 32];
+  const int nvec = dim / 8;
+  const size_t base = static_cast<size_t>(blockIdx.x) * dim;
+  const uint4* x = reinterpret_cast<const uint4*>(X + base);
+  uint4 v[VPT];
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    v[i] = j < nvec ? __ldcs(x + j) : make_uint4(0, 0, 0, 0);
+  }
+  // magnitudes compare like their bits, and those of infinities and NaNs lie above all numbers
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = __vmaxu2(top, u[k] & 0x7fff7fffu);
+  }
+  top = max(top & 0xffffu, top >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t* r = reinterpret_cast<uint32_t*>(red);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockDim.x > 32) {
+    if (lane == 0) r[warp] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < static_cast<int>(blockDim.x >> 5) ? r[lane] : 0u);
+  }
+  const bool finite = top < (BF16 ? 0x7f80u : 0x7c00u);
+  const float amax = fmaxf(unpack2<BF16>(top).x, 0x1p-100f);
+  const float inv = __fdiv_rn(127.f, amax);
+  if (threadIdx.x == 0) S[blockIdx.x] = finite ? __fdiv_rn(amax, 127.f) : __int_as_float(0x7fc00000);
+  uint2* q = reinterpret_cast<uint2*>(Q + base);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = threadIdx.x + i * blockDim.x;
+    if (j < nvec) {
+      const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t b[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2<BF16>(u[k]);
+        // (at most 127 in magnitude: the quotient's rounding is less than half a step there)
+        b[2 * k] = finite ? static_cast<uint32_t>(__float2int_rn(__fmul_rn(f.x, inv))) & 0xffu : 0u;
+        b[2 * k + 1] = finite ? static_cast<uint32_t>(__float2int_rn(__fmul_rn(f.y, inv))) & 0xffu : 0u;
+      }
+      q[j] = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+    }
+  }
+}
+
+template <bool BF16, int VPT>
+cudaError_t launch_quantize(const uint16_t* x, int8_t* q, float* s, int rows, int dim, cudaStream_t stream) {
+  const int nvec = dim / 8;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows, 1, 1);
+  cfg.blockDim = dim3(((nvec + VPT - 1) / VPT + 31) / 32 * 32, 1, 1);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_rows_kernel<BF16, VPT>, x, q, s, dim);
+  if (e != cudaSuccess) cudaGetLastError();  // reported to the caller, not left for the next one
+  return e;
+}
+
+template <bool BF16>
+cudaError_t quantize(const uint16_t* x, int8_t* q, float* s, int rows, int dim, cudaStream_t stream) {
+  const int nvec = dim / 8;
+  if (nvec <= kQuantizeThreads / 2) return launch_quantize<BF16, 1>(x, q, s, rows, dim, stream);
+  if (nvec <= kQuantizeThreads) return launch_quantize<BF16, 2>(x, q, s, rows, dim, stream);
+  if (nvec <= 2 * kQuantizeThreads) return launch_quantize<BF16, 4>(x, q, s, rows, dim, stream);
+  return launch_quantize<BF16, 8>(x, q, s, rows, dim, stream);
+}
+
 }  // namespace
+
+cudaError_t quantize_rows_launch(const void* X, void* Q, float* S, int rows, int dim, bool bf16, cudaStream_t stream) {
+  if (dim < 8 || dim % 8 != 0 || dim > kMaxQuantizeDim) return cudaErrorInvalidValue;
+  if (rows == 0) return cudaSuccess;
+  const uint16_t* x = static_cast<const uint16_t*>(X);
+  int8_t* q = static_cast<int8_t*>(Q);
+  return bf16 ? quantize<true>(x, q, S, rows, dim, stream) : quantize<false>(x, q, S, rows, dim, stream);
+}
 
 cudaError_t rope_launch(void* QKV, int tokens, int seq, int heads, int head_dim, int row_elems, float theta, bool bf16,
                         cudaStream_t stream) {

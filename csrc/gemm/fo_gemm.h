@@ -17,6 +17,11 @@ namespace fo {
 std::string encode_tmap_16bit(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
                               uint32_t box_rows);
 
+// The same over [batch, rows, cols] 8-bit elements with a (1 x box_rows x 128) box: 3-D if batched, so that rows past one
+// matrix's last are zeros and not the next one's, else 2-D with batch 1.  cols must be a multiple of 16.
+std::string encode_tmap_8bit(CUtensorMap* out, const void* ptr, uint64_t batch, uint64_t rows, uint64_t cols,
+                             uint32_t box_rows, bool batched);
+
 // Fills tiles_m / tiles_n / num_tiles / raster_sw of `p` for `algo` and checks divisibility.
 std::string prepare_tiling(int algo, GemmParams* p);
 

@@ -1,0 +1,156 @@
+// Instantiations of the 8-bit GEMM kernels and the choice between them.
+#include "fo_gemm.h"
+#include "fo_gemm_i8.h"
+#include "fo_gemm_i8_sm100.cuh"
+
+#include <algorithm>
+
+namespace fo {
+
+namespace {
+
+template <typename Kernel>
+cudaError_t prepare(Kernel kernel, int smem, bool* attr_set) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 16 && attr_set[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev >= 0 && dev < 16) attr_set[dev] = true;
+  return e;
+}
+
+cudaLaunchConfig_t config(int64_t grid, int threads, int smem, int cluster, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cfg;
+}
+
+// CTA pairs of the wide kernel that run at once on the current device.
+template <bool BF16, bool GROUPED>
+int resident_pairs() {
+  static int cache[16] = {};  // 0: not asked yet
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16) return 1;
+  if (cache[dev] == 0) {
+    int sm_count = 0, clusters = 0;
+    cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = config(sm_count & ~1, kI8WideThreads, I8WideSmem<GROUPED>::kTotalBytes, 2, nullptr, attr);
+    cfg.attrs = attr + 1;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&clusters, fo_gemm_i8_wide_kernel<BF16, GROUPED>, &cfg) != cudaSuccess || clusters < 1) {
+      cudaGetLastError();
+      clusters = 1;
+    }
+    cache[dev] = clusters;
+  }
+  return cache[dev];
+}
+
+template <bool BF16, bool GROUPED>
+cudaError_t launch_wide(const GemmI8Maps& maps, const GemmI8Params& p, cudaStream_t stream) {
+  constexpr int smem = I8WideSmem<GROUPED>::kTotalBytes;
+  static_assert(smem <= 227 * 1024, "shared memory of this configuration exceeds 227 KB");
+  static bool attr_set[16] = {};
+  auto kernel = fo_gemm_i8_wide_kernel<BF16, GROUPED>;
+  const cudaError_t e = prepare(kernel, smem, attr_set);
+  if (e != cudaSuccess) return e;
+  // with offsets, every expert may end in a tile of its own
+  const int64_t units = ((p.M + kI8Rows - 1) / kI8Rows + (GROUPED ? std::min(p.experts, p.M) : 0)) * static_cast<int64_t>(p.tiles_n);
+  const int64_t pairs = std::min<int64_t>(units, resident_pairs<BF16, GROUPED>());
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config(2 * pairs, kI8WideThreads, smem, 2, stream, attr);
+  return cudaLaunchKernelEx(&cfg, kernel, maps, p);
+}
+
+template <bool BF16, int TN, int S>
+cudaError_t launch_narrow(const GemmI8Maps& maps, const GemmI8Params& p, cudaStream_t stream) {
+  constexpr int smem = I8NarrowSmem<TN, S>::kTotalBytes;
+  static_assert(smem <= 227 * 1024, "shared memory of this configuration exceeds 227 KB");
+  static bool attr_set[16] = {};
+  auto kernel = fo_gemm_i8_narrow_kernel<BF16, TN, S>;
+  const cudaError_t e = prepare(kernel, smem, attr_set);
+  if (e != cudaSuccess) return e;
+  const int64_t grid = static_cast<int64_t>(p.token_tiles) * ((p.N + 127) / 128) * S;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config(grid, kI8NarrowThreads, smem, S, stream, attr);
+  return cudaLaunchKernelEx(&cfg, kernel, maps, p);
+}
+
+template <bool BF16, int TN>
+cudaError_t dispatch_split(int split, const GemmI8Maps& maps, const GemmI8Params& p, cudaStream_t stream) {
+  switch (split) {
+    case 1: return launch_narrow<BF16, TN, 1>(maps, p, stream);
+    case 2: return launch_narrow<BF16, TN, 2>(maps, p, stream);
+    case 4: return launch_narrow<BF16, TN, 4>(maps, p, stream);
+    default: break;
+  }
+  if constexpr (TN >= 32) {
+    if (split == 8) return launch_narrow<BF16, TN, 8>(maps, p, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+template <bool BF16>
+cudaError_t dispatch(const GemmI8Plan& plan, const GemmI8Maps& maps, const GemmI8Params& p, cudaStream_t stream) {
+  switch (plan.tokens) {
+    case 0: return p.offsets != nullptr ? launch_wide<BF16, true>(maps, p, stream) : launch_wide<BF16, false>(maps, p, stream);
+    case 16: return dispatch_split<BF16, 16>(plan.split, maps, p, stream);
+    case 32: return dispatch_split<BF16, 32>(plan.split, maps, p, stream);
+    case 64: return dispatch_split<BF16, 64>(plan.split, maps, p, stream);
+    case 128: return dispatch_split<BF16, 128>(plan.split, maps, p, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+GemmI8Plan choose_i8(int M, int N, int K, int experts, bool grouped) {
+  GemmI8Plan plan{0, 1};
+  const int per = grouped ? (M + experts - 1) / experts : M;  // tokens of a weight matrix
+  if (per > 128) return plan;
+  plan.tokens = per <= 16 ? 16 : per <= 32 ? 32 : per <= 64 ? 64 : 128;
+  const int64_t tiles = static_cast<int64_t>((N + 127) / 128) * (grouped ? std::min(experts, M) : 1);
+  const int num_kb = (K + kI8BK - 1) / kI8BK;
+  const int slots = plan.tokens == 128 ? 148 : 296;
+  while (plan.split < 8 && plan.split * 2 * 4 <= plan.tokens && tiles * plan.split * 2 <= slots && num_kb >= plan.split * 4) plan.split *= 2;
+  return plan;
+}
+
+std::string gemm_i8_launch(const GemmI8Plan& plan, GemmI8Params p, const void* A, const void* B, bool bf16,
+                           cudaStream_t stream) {
+  GemmI8Maps maps;
+  const bool wide = plan.tokens == 0;
+  std::string e = encode_tmap_8bit(&maps.a, A, 1, p.M, p.K, wide ? 128 : plan.tokens, false);
+  if (!e.empty()) return "A: " + e;
+  e = encode_tmap_8bit(&maps.b, B, p.experts, p.N, p.K, 128, true);
+  if (!e.empty()) return "B: " + e;
+  e = encode_tmap_16bit(&maps.c, p.C, p.M, p.N, 32);
+  if (!e.empty()) return "C: " + e;
+  p.tiles_n = (p.N + kI8Cols - 1) / kI8Cols;
+  p.raster_sw = std::min(8, p.tiles_n);
+  if (!wide) {
+    // with offsets: the tiles that the rows can have at most, one more than they fill for each expert
+    p.token_tiles = p.offsets == nullptr ? (p.M + plan.tokens - 1) / plan.tokens
+                                         : p.M / plan.tokens + std::min(p.experts, p.M);
+  }
+  const cudaError_t r = bf16 ? dispatch<true>(plan, maps, p, stream) : dispatch<false>(plan, maps, p, stream);
+  if (r == cudaSuccess) return "";
+  cudaGetLastError();  // reported to the caller, not left for the next one
+  return std::string("launch: ") + cudaGetErrorString(r);
+}
+
+}  // namespace fo

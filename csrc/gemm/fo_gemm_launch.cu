@@ -118,6 +118,23 @@ std::string encode_tmap_16bit(CUtensorMap* out, const void* ptr, uint64_t rows, 
   return "";
 }
 
+std::string encode_tmap_8bit(CUtensorMap* out, const void* ptr, uint64_t batch, uint64_t rows, uint64_t cols,
+                             uint32_t box_rows, bool batched) {
+  EncodeFn fn = get_encode_fn();
+  if (fn == nullptr) return "cuTensorMapEncodeTiled is not available from this driver";
+  if ((reinterpret_cast<uintptr_t>(ptr) & 15u) != 0) return "operand is not 16-byte aligned";
+  if (cols % 16 != 0) return "row pitch is not a multiple of 16 bytes";
+  cuuint64_t dims[3] = {cols, rows, batch};
+  cuuint64_t strides[2] = {cols, cols * rows};
+  cuuint32_t box[3] = {128, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, batched ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return "cuTensorMapEncodeTiled failed with code " + std::to_string(int(r));
+  return "";
+}
+
 std::string prepare_tiling(int algo, GemmParams* p) {
   if (algo < 0 || algo >= kNumAlgos) return "Algo index out of range";
   const AlgoConfig c = algo_config(algo);

@@ -1,0 +1,428 @@
+// Rows sorted by expert and back.  A router gives every token top_k experts; the products run on each expert's rows
+// together, so a token's row is copied to top_k places of a matrix sorted by expert, and afterwards the
+// top_k results are summed with the router's weights.  All sums are fp32; there are no atomics on global
+// memory, and every result is the same from call to call.
+#include "fo_moe.h"
+
+#include <algorithm>
+
+#include "../common/fo_pack16.cuh"
+#include "../common/fo_ptx.cuh"
+
+namespace fo {
+
+namespace {
+
+// ---------------------------------------------------------------------------- the order
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortCluster = 8;
+
+__device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// A stable counting sort in one launch: one CTA, or a cluster of eight.  Every warp takes a run of choices: it counts
+// them by expert in a row of its own in shared memory (lanes with equal experts find each other by
+// match.any), the counts of the warps and, through distributed shared memory, of the CTAs in front of it give
+// each warp its first row for every expert, and a second walk over the same run hands the rows out.
+// Bound by latency: the walks are chains of shared-memory updates, 32 choices a step.
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads)
+    moe_sort_kernel(const Id* __restrict__ ids, int64_t n, int experts, int32_t* __restrict__ slot,
+                    int32_t* __restrict__ source, int32_t* __restrict__ offsets) {
+  extern __shared__ uint32_t smem[];
+  uint32_t* count = smem;                       // [kSortWarps][experts], then the next row of each
+  uint32_t* total = count + kSortWarps * experts;  // [experts]: this CTA's choices
+  __shared__ uint32_t scan[kSortWarps];
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int ctas = static_cast<int>(gridDim.x);  // one cluster
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t* mine = count + warp * experts;
+  for (int e = threadIdx.x; e < kSortWarps * experts; e += kSortThreads) count[e] = 0;
+  const int64_t per_warp = (n + ctas * kSortThreads - 1) / (ctas * kSortThreads) * 32;
+  const int64_t begin = min(n, (static_cast<int64_t>(rank) * kSortWarps + warp) * per_warp);
+  const int64_t end = min(n, begin + per_warp);
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+  __syncthreads();
+  // expert of choice i; `experts` for a choice without one and for lanes past the end
+  auto expert_at = [&](int64_t i) -> int {
+    if (i >= end) return experts;
+    const Id v = ids[i];
+    return v >= 0 && v < static_cast<Id>(experts) ? static_cast<int>(v) : experts;
+  };
+  int next = expert_at(begin + lane);
+  for (int64_t i = begin; i < end; i += 32) {
+    const int e = next;
+    next = expert_at(i + 32 + lane);
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    if (e < experts && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  const int e = threadIdx.x;  // experts <= kSortThreads
+  if (e < experts) {
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t c = count[w * experts + e];
+      count[w * experts + e] = sum;
+      sum += c;
+    }
+    total[e] = sum;
+  }
+  __syncwarp();  // the barrier's aligned forms take whole warps
+  ptx::cluster_arrive_release();
+  ptx::cluster_wait_acquire();
+  uint32_t before = 0, all = 0;
+  if (e < experts) {
+    for (int c = 0; c < ctas; ++c) {
+      const uint32_t v = ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(total + e), c));
+      if (c < rank) before += v;
+      all += v;
+    }
+  }
+  // nobody reads another CTA's counts from here on
+  __syncwarp();
+  ptx::cluster_arrive_relaxed();
+  // exclusive sums over the experts
+  uint32_t incl = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  uint32_t warps = scan[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, warps, o);
+    if (lane >= o) warps += v;
+  }
+  const uint32_t rows = __shfl_sync(0xffffffffu, warps, 31);
+  const uint32_t in_front = __shfl_sync(0xffffffffu, warps, warp > 0 ? warp - 1 : 0);
+  const uint32_t first = incl - all + (warp > 0 ? in_front : 0u);
+  if (e < experts) {
+    if (rank == 0) offsets[e] = static_cast<int32_t>(first);
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) count[w * experts + e] += first + before;
+  }
+  if (rank == 0 && threadIdx.x == 0) offsets[experts] = static_cast<int32_t>(rows);
+  __syncthreads();
+  next = expert_at(begin + lane);
+  for (int64_t i = begin; i < end; i += 32) {
+    const int ex = next;
+    next = expert_at(i + 32 + lane);
+    const uint32_t same = __match_any_sync(0xffffffffu, ex);
+    int32_t row = -1;
+    if (ex < experts) {
+      row = static_cast<int32_t>(mine[ex] + __popc(same & ((1u << lane) - 1u)));
+      source[row] = static_cast<int32_t>(i + lane);
+    }
+    __syncwarp();
+    if (ex < experts && lane == __ffs(same) - 1) mine[ex] += __popc(same);
+    __syncwarp();
+    if (i + lane < end) slot[i + lane] = row;
+  }
+  for (int64_t r = rows + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n; r += static_cast<int64_t>(ctas) * kSortThreads) {
+    source[r] = -1;
+  }
+  __syncwarp();
+  ptx::cluster_wait_acquire();
+}
+
+// ---------------------------------------------------------------------------- the rows
+
+constexpr int kRowThreads = 256;
+
+// The row of a choice if it is one of the `rows` there are, else -1: an order made for something else is not followed
+// out of the matrix.
+__device__ __forceinline__ int row_at(const int32_t* slot, int64_t choice, int64_t rows) {
+  const int row = slot[choice];
+  return static_cast<uint32_t>(row) < static_cast<uint32_t>(rows) ? row : -1;
+}
+
+// The rows behind the last expert's, zeroed by all threads of the grid.
+__device__ __forceinline__ void zero_rows(uint4* rows, int64_t first, int64_t last, int nvec) {
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t end = last * nvec;
+  for (int64_t v = max(first, static_cast<int64_t>(0)) * nvec + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < end; v += step) rows[v] = zero;
+}
+
+// Bound by the rows written: every token's row is read once.  A thread copies one vector of a token to its top_k rows.
+__global__ void __launch_bounds__(kRowThreads)
+    moe_dispatch_kernel(const uint4* __restrict__ X, const int32_t* __restrict__ slot,
+                        const int32_t* __restrict__ offsets, uint4* __restrict__ R, int tokens, int top_k, int nvec,
+                        int experts) {
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+  const int64_t token = v / nvec;
+  if (token < tokens) {
+    const int j = static_cast<int>(v - token * nvec);
+    const uint4 x = __ldcs(X + v);
+    const int64_t rows = static_cast<int64_t>(tokens) * top_k;
+#pragma unroll 4
+    for (int k = 0; k < top_k; ++k) {
+      const int row = row_at(slot, token * top_k + k, rows);
+      if (row >= 0) R[static_cast<int64_t>(row) * nvec + j] = x;
+    }
+  }
+  zero_rows(R, offsets[experts], static_cast<int64_t>(tokens) * top_k, nvec);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float weight_at(const void* w, bool f32, int64_t i) {
+  if (w == nullptr) return 1.f;
+  if (f32) return static_cast<const float*>(w)[i];
+  if constexpr (BF16) {
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+  } else {
+    return __half2float(static_cast<const __half*>(w)[i]);
+  }
+}
+
+constexpr int kUnrollK = 8;  // rows of a token in flight per thread
+
+// Bound by the rows read.  A thread sums one vector of a token over its top_k rows, in their order.
+template <bool BF16>
+__global__ void __launch_bounds__(kRowThreads)
+    moe_combine_kernel(const uint4* __restrict__ R, const void* __restrict__ w, bool f32,
+                       const int32_t* __restrict__ slot, uint4* __restrict__ O, int tokens, int top_k, int nvec) {
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+  const int64_t token = v / nvec;
+  if (token >= tokens) return;
+  const int j = static_cast<int>(v - token * nvec);
+  const int64_t rows = static_cast<int64_t>(tokens) * top_k;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  for (int k0 = 0; k0 < top_k; k0 += kUnrollK) {
+    uint4 r[kUnrollK];
+    int row[kUnrollK];
+#pragma unroll
+    for (int k = 0; k < kUnrollK; ++k) row[k] = k0 + k < top_k ? row_at(slot, token * top_k + k0 + k, rows) : -1;
+#pragma unroll
+    for (int k = 0; k < kUnrollK; ++k) {
+      if (row[k] >= 0) r[k] = __ldcs(R + static_cast<int64_t>(row[k]) * nvec + j);
+    }
+#pragma unroll
+    for (int k = 0; k < kUnrollK; ++k) {
+      if (row[k] >= 0) {
+        const float wk = weight_at<BF16>(w, f32, token * top_k + k0 + k);
+        const uint32_t u[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack2<BF16>(u[i]);
+          acc[2 * i] += wk * f.x;
+          acc[2 * i + 1] += wk * f.y;
+        }
+      }
+    }
+  }
+  O[v] = make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]),
+                    pack2<BF16>(acc[6], acc[7]));
+}
+
+// Bound by memory: the token's gradient is read once, every row of the experts is read (for its weight's gradient) and its
+// gradient written.  A CTA takes a token; the dots are summed over its threads in a fixed order.
+template <bool BF16, bool ROWS, bool WEIGHTS>
+__global__ void __launch_bounds__(kRowThreads)
+    moe_combine_backward_kernel(const uint4* __restrict__ GO, const uint4* __restrict__ R, const void* __restrict__ w,
+                                bool f32, const int32_t* __restrict__ slot, const int32_t* __restrict__ offsets,
+                                uint4* __restrict__ DR, void* __restrict__ DW, int tokens, int top_k, int nvec,
+                                int experts) {
+  __shared__ float part[kRowThreads / 32][kUnrollK];
+  const int64_t token = blockIdx.x;
+  const int64_t rows = static_cast<int64_t>(tokens) * top_k;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+  for (int k0 = 0; k0 < top_k; k0 += kUnrollK) {
+    int row[kUnrollK];
+    float wk[kUnrollK], dot[kUnrollK];
+#pragma unroll
+    for (int k = 0; k < kUnrollK; ++k) {
+      row[k] = k0 + k < top_k ? row_at(slot, token * top_k + k0 + k, rows) : -1;
+      dot[k] = 0.f;
+      wk[k] = ROWS && row[k] >= 0 ? weight_at<BF16>(w, f32, token * top_k + k0 + k) : 0.f;
+    }
+    for (int j = threadIdx.x; j < nvec; j += blockDim.x) {
+      const uint4 g = __ldg(GO + token * nvec + j);
+      uint4 r[kUnrollK];
+      if constexpr (WEIGHTS) {
+#pragma unroll
+        for (int k = 0; k < kUnrollK; ++k) {
+          if (row[k] >= 0) r[k] = __ldcs(R + static_cast<int64_t>(row[k]) * nvec + j);
+        }
+      }
+      const uint32_t gu[4] = {g.x, g.y, g.z, g.w};
+      float gf[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<BF16>(gu[i]);
+        gf[2 * i] = f.x;
+        gf[2 * i + 1] = f.y;
+      }
+#pragma unroll
+      for (int k = 0; k < kUnrollK; ++k) {
+        if (row[k] < 0) continue;
+        if constexpr (WEIGHTS) {
+          const uint32_t u[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<BF16>(u[i]);
+            dot[k] += gf[2 * i] * f.x + gf[2 * i + 1] * f.y;
+          }
+        }
+        if constexpr (ROWS) {
+          uint4 d;
+          d.x = pack2<BF16>(wk[k] * gf[0], wk[k] * gf[1]);
+          d.y = pack2<BF16>(wk[k] * gf[2], wk[k] * gf[3]);
+          d.z = pack2<BF16>(wk[k] * gf[4], wk[k] * gf[5]);
+          d.w = pack2<BF16>(wk[k] * gf[6], wk[k] * gf[7]);
+          __stcs(DR + static_cast<int64_t>(row[k]) * nvec + j, d);
+        }
+      }
+    }
+    if constexpr (WEIGHTS) {
+#pragma unroll
+      for (int k = 0; k < kUnrollK; ++k) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+      }
+      __syncthreads();  // the previous round's sums have been read
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < kUnrollK; ++k) part[warp][k] = dot[k];
+      }
+      __syncthreads();
+      const int k = threadIdx.x;
+      if (k < kUnrollK && k0 + k < top_k) {
+        float s = 0.f;
+        for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) s += part[i][k];
+        const int64_t at = token * top_k + k0 + k;
+        if (f32) {
+          static_cast<float*>(DW)[at] = s;
+        } else if constexpr (BF16) {
+          static_cast<__nv_bfloat16*>(DW)[at] = __float2bfloat16_rn(s);
+        } else {
+          static_cast<__half*>(DW)[at] = __float2half_rn(s);
+        }
+      }
+    }
+  }
+  if constexpr (ROWS) zero_rows(DR, offsets[experts], static_cast<int64_t>(tokens) * top_k, nvec);
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel kernel, int64_t grid, int threads, cudaStream_t stream, Args... args) {
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) cudaGetLastError();  // reported to the caller, not left for the next one
+  return e;
+}
+
+template <typename Id>
+cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, int32_t* source, int32_t* offsets,
+                        cudaStream_t stream) {
+  auto kernel = moe_sort_kernel<Id>;
+  const int smem = (kSortWarps + 1) * experts * static_cast<int>(sizeof(uint32_t));
+  static bool set[16] = {};  // the same whoever sets it
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16 || !set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (kSortWarps + 1) * kMaxExperts * static_cast<int>(sizeof(uint32_t)));
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 16) set[dev] = true;
+  }
+  const int ctas = n <= 4 * kSortThreads ? 1 : kSortCluster;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.blockDim = dim3(kSortThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), n, experts, slot, source, offsets);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e;
+}
+
+bool valid(const MoeShape& s) {
+  return s.tokens >= 1 && s.top_k >= 1 && s.top_k <= kMaxTopK && s.dim >= 8 && s.dim % 8 == 0 && s.experts >= 1 &&
+         s.experts <= kMaxExperts && static_cast<int64_t>(s.tokens) * s.top_k <= INT32_MAX;
+}
+
+int64_t vec_ctas(const MoeShape& s) { return (static_cast<int64_t>(s.tokens) * (s.dim / 8) + kRowThreads - 1) / kRowThreads; }
+
+template <bool BF16>
+cudaError_t launch_backward(const MoeShape& s, const uint4* go, const uint4* r, MoeWeights w, const int32_t* slot,
+                            const int32_t* offsets, uint4* dr, void* dw, cudaStream_t stream) {
+  const int nvec = s.dim / 8;
+  const int threads = std::min(kRowThreads, (nvec + 31) / 32 * 32);
+  auto kernel = dr == nullptr ? moe_combine_backward_kernel<BF16, false, true>
+                : dw == nullptr ? moe_combine_backward_kernel<BF16, true, false>
+                                : moe_combine_backward_kernel<BF16, true, true>;
+  return launch(kernel, s.tokens, threads, stream, go, r, w.p, w.f32, slot, offsets, dr, dw, s.tokens, s.top_k, nvec, s.experts);
+}
+
+}  // namespace
+
+cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int experts, int32_t* slot, int32_t* source,
+                            int32_t* offsets, cudaStream_t stream) {
+  if (experts < 1 || experts > kMaxExperts || choices < 0 || choices > INT32_MAX) return cudaErrorInvalidValue;
+  return ids64 ? launch_sort<int64_t>(ids, choices, experts, slot, source, offsets, stream)
+               : launch_sort<int32_t>(ids, choices, experts, slot, source, offsets, stream);
+}
+
+cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t* slot, const int32_t* offsets, void* R,
+                                cudaStream_t stream) {
+  if (!valid(s)) return cudaErrorInvalidValue;
+  return launch(moe_dispatch_kernel, vec_ctas(s), kRowThreads, stream, static_cast<const uint4*>(X), slot, offsets,
+                static_cast<uint4*>(R), s.tokens, s.top_k, s.dim / 8, s.experts);
+}
+
+cudaError_t moe_combine_launch(const MoeShape& s, const void* R, MoeWeights w, const int32_t* slot, void* O,
+                               cudaStream_t stream) {
+  if (!valid(s)) return cudaErrorInvalidValue;
+  return launch(s.bf16 ? moe_combine_kernel<true> : moe_combine_kernel<false>, vec_ctas(s), kRowThreads, stream,
+                static_cast<const uint4*>(R), w.p, w.f32, slot, static_cast<uint4*>(O), s.tokens, s.top_k, s.dim / 8);
+}
+
+cudaError_t moe_combine_backward_launch(const MoeShape& s, const void* GO, const void* R, MoeWeights w,
+                                        const int32_t* slot, const int32_t* offsets, void* DR, void* DW,
+                                        cudaStream_t stream) {
+  if (!valid(s) || (DR == nullptr && DW == nullptr)) return cudaErrorInvalidValue;
+  const uint4 *go = static_cast<const uint4*>(GO), *r = static_cast<const uint4*>(R);
+  uint4* dr = static_cast<uint4*>(DR);
+  return s.bf16 ? launch_backward<true>(s, go, r, w, slot, offsets, dr, DW, stream)
+                : launch_backward<false>(s, go, r, w, slot, offsets, dr, DW, stream);
+}
+
+}  // namespace fo

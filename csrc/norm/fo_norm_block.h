@@ -1,0 +1,34 @@
+// Host launchers of the norms around a block (no counterpart in the reference):
+//   u = rmsnorm(T) * PW,  H = alpha * X + G u,  Y = rmsnorm(H) * W      with r1, r2 the two rows' 1 / rms.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace fo {
+
+// One call's operands: 16-bit row-major [rows, dim], weights [dim], gate [lines, dim] (lines consecutive groups of
+// rows / lines rows share a line; nullptr: no gate), stats [rows][2] fp32 = (r1, r2).
+struct NormBlock {
+  const void *X, *T, *PW, *W, *G;
+  int rows, dim, lines;
+  float alpha, eps;
+  bool bf16;
+};
+
+// stats may be nullptr.
+cudaError_t norm_block_launch(const NormBlock& p, void* H, void* Y, float* stats, int sm_count, cudaStream_t stream);
+
+// How the rows are dealt out in the backward pass: `chunks` runs of rows for every line of the gate (1 without a
+// gate, or with one line: the CTAs' own runs), `ctas` CTAs.
+struct NormBlockPlan {
+  int ctas, chunks;
+  size_t workspace;  // floats
+};
+NormBlockPlan norm_block_plan(const NormBlock& p, int sm_count);
+
+// GH, GY: gradients of H and Y (either may be nullptr: zero).  DX, DT [rows, dim], DPW, DW [dim], DG like G
+// (ignored without a gate).  `workspace`: plan.workspace floats.
+cudaError_t norm_block_backward_launch(const NormBlock& p, const float* stats, const void* GH, const void* GY, void* DX,
+                                       void* DT, void* DPW, void* DW, void* DG, float* workspace,
+                                       const NormBlockPlan& plan, cudaStream_t stream);
+
+}  // namespace fo

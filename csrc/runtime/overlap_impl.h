@@ -72,6 +72,12 @@ class OverlapImpl : public torch::CustomClassHolder {
   //   C <- silu(A * G^T) * (A * U^T)   B = [G; U], G and U [N, K] each, C [M, N]
   void GemmAdd(at::Tensor A, at::Tensor B, at::Tensor R, at::Tensor C, int64_t Algo);
   void GemmSwiGLU(at::Tensor A, at::Tensor B, at::Tensor C);
+  // Single-rank product of 8-bit integers with a scale for each token and each channel (gemm/fo_gemm_i8.h):
+  //   C[m, n] <- SA[m] * SB[n] * sum_k A[m, k] * B[n, k]       A [M, K], B [N, K] int8, SA [M], SB [N] fp32
+  // and by expert, B [experts, N, K], SB [experts, N]: rows offsets[e] .. offsets[e + 1] - 1 times B[e], other rows zero.
+  void GemmI8(at::Tensor A, at::Tensor B, at::Tensor SA, at::Tensor SB, at::Tensor C, c10::optional<at::Tensor> offsets);
+  // The same of 16-bit activations X [..., K], brought to 8 bits row by row first; returns [..., N] in X's type.
+  at::Tensor LinearI8(at::Tensor X, at::Tensor B, at::Tensor SB, c10::optional<at::Tensor> offsets);
   // GEMM whose epilogue stores every row of A * B^T straight into the receive buffer D of the
   // rank it is bound for, over NVLink; same row bookkeeping as gemm_all2all (mLen_CPU[r][i]
   // rows go from rank r to rank i, runs packed in rank order, own run excluded), no C and no

@@ -32,7 +32,10 @@ SOURCES = [
     "gemm/fo_gemm_launch.cu",
     "gemm/fo_gemm_plain_launch.cu",
     "gemm/fo_gemm_splitk_launch.cu",
+    "gemm/fo_gemm_i8_launch.cu",
     "norm/fo_norm.cu",
+    "norm/fo_norm_block.cu",
+    "moe/fo_moe.cu",
     "elementwise/fo_elementwise.cu",
     "flags/fo_wait.cu",
     "noalloc/fo_noalloc.cu",

@@ -11,6 +11,9 @@ from typing import List, Optional, Sequence
 import torch
 
 from .._build import load as _load
+from .experts import ExpertOrder, moe_combine, moe_dispatch, moe_sort  # noqa: F401
+from .linear_i8 import linear_i8, quantize_rows  # noqa: F401
+from .norm_block import rmsnorm_add_rmsnorm  # noqa: F401
 
 
 def _op():
