@@ -4,6 +4,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
@@ -130,6 +132,29 @@ void check_16bit(const at::Tensor& t, const char* name) {
 }
 
 bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return given(t) ? *t : at::Tensor(); }
+c10::optional<at::Tensor> or_none(const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
+
+// The operators with gradients.  They are functions of their own on torch's tape, in C++: a step through a pair of them
+// from Python (two calls and one backward pass of few rows) is bound by the host, and the interpreter would be most of that.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+template <typename... T>
+bool records(const T&... t) {
+  return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
+}
+
+// Gradients whose own derivatives do not exist: with a graph being recorded for them, differentiating it raises.
+variable_list once(const char* name, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative",
+                                                               static_cast<int64_t>(grads.size()));
+  for (at::Tensor& g : grads) {
+    if (g.defined()) g = g.detach().requires_grad_();
+  }
+  return (*error)(std::move(grads));
+}
 
 // The operands of rmsnorm_add_rmsnorm and of its backward pass, checked.
 struct NormBlockOperands {
@@ -173,9 +198,9 @@ NormBlockOperands norm_block_operands(const at::Tensor& X, const at::Tensor& T, 
 
 // (H, Y, stats): u = rmsnorm(T) * PW, H = alpha * X + G * u, Y = rmsnorm(H) * W; stats [rows, 2] fp32 (1 / rms of T and of H),
 // what the backward pass needs, if asked for, else empty.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_add_rmsnorm(at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
-                                                                    c10::optional<at::Tensor> G, double alpha, double eps,
-                                                                    bool with_stats) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_block_forward(at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
+                                                                  c10::optional<at::Tensor> G, double alpha, double eps,
+                                                                  bool with_stats) {
   check_16bit(X, "X");
   c10::cuda::CUDAGuard guard(X.device());
   const NormBlockOperands o = norm_block_operands(X, T, PW, W, G, alpha, eps);
@@ -223,6 +248,40 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm_a
                    "rmsnorm_add_rmsnorm_backward");
   }
   return {DX, DT, DPW, DW, DG};
+}
+
+struct NormBlockFunction : public torch::autograd::Function<NormBlockFunction> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
+                               c10::optional<at::Tensor> G, double alpha, double eps) {
+    auto [H, Y, stats] = norm_block_forward(X, T, PW, W, G, alpha, eps, true);
+    ctx->save_for_backward({X, T, PW, W, or_undefined(G), stats});
+    ctx->saved_data["alpha"] = alpha;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({stats});
+    return {H, Y, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(7);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list v = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [DX, DT, DPW, DW, DG] = rmsnorm_add_rmsnorm_backward(or_none(grads[0]), or_none(grads[1]), v[0], v[1], v[2], v[3],
+                                                              or_none(v[4]), v[5], ctx->saved_data["alpha"].toDouble());
+    const at::Tensor all[5] = {DX, DT, DPW, DW, DG};
+    for (int i = 0; i < 5; ++i) {
+      if (v[i].defined() && ctx->needs_input_grad(i)) out[i] = all[i];
+    }
+    return once("rmsnorm_add_rmsnorm", std::move(out));
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_add_rmsnorm(at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
+                                                                    c10::optional<at::Tensor> G, double alpha, double eps,
+                                                                    bool with_stats) {
+  const at::Tensor g = or_undefined(G);
+  if (!records(X, T, PW, W, g)) return norm_block_forward(X, T, PW, W, G, alpha, eps, with_stats);
+  const variable_list out = NormBlockFunction::apply(X, T, PW, W, or_none(g), alpha, eps);
+  return {out[0], out[1], out[2]};
 }
 
 // (slot [tokens, top_k], source [tokens * top_k], offsets [experts + 1]) of the experts `ids` [tokens, top_k] chosen for each token.
@@ -277,7 +336,7 @@ fo::MoeWeights weights_arg(const at::Tensor& w) {
 }
 
 // R [tokens * top_k, dim]: R[slot[t, k]] = X[t], the rows behind the last expert's zero.
-at::Tensor moe_dispatch(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
+at::Tensor dispatch_rows(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
   check_16bit(X, "X");
   FO_CHECK(X.dim() == 2 && slot.dim() == 2 && X.size(0) == slot.size(0), "X must be [tokens, dim] and slot [tokens, top_k]");
   c10::cuda::CUDAGuard guard(X.device());
@@ -293,11 +352,11 @@ at::Tensor moe_dispatch(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
 }
 
 // O [tokens, dim]: the sum over k of weights[t, k] * R[slot[t, k]] (no weights: 1).
-at::Tensor moe_combine(at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot) {
+at::Tensor combine_rows(at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot, const at::Tensor* offsets) {
   check_16bit(R, "R");
   FO_CHECK(R.dim() == 2 && R.size(0) == slot.numel(), "R must be [tokens * top_k, dim] and slot [tokens, top_k]");
   c10::cuda::CUDAGuard guard(R.device());
-  const fo::MoeShape s = moe_shape(R, R.size(1), slot, nullptr);
+  const fo::MoeShape s = moe_shape(R, R.size(1), slot, offsets);
   const at::Tensor r = dense(R), w = moe_weights(weights, R, slot);
   at::Tensor O = at::empty({slot.size(0), R.size(1)}, r.options());
   if (s.tokens > 0) {
@@ -336,6 +395,48 @@ std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::opti
                    "moe_combine_backward");
   }
   return {DR, DW};
+}
+
+struct DispatchFunction : public torch::autograd::Function<DispatchFunction> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor X, at::Tensor slot, at::Tensor offsets) {
+    ctx->save_for_backward({slot});
+    return dispatch_rows(X, slot, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list v = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
+    return once("moe_dispatch", {combine_rows(grads[0], c10::nullopt, v[0], nullptr), at::Tensor(), at::Tensor()});
+  }
+};
+
+at::Tensor moe_dispatch(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
+  return records(X) ? DispatchFunction::apply(X, slot, offsets) : dispatch_rows(X, slot, offsets);
+}
+
+struct CombineFunction : public torch::autograd::Function<CombineFunction> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot,
+                            at::Tensor offsets) {
+    const at::Tensor w = or_undefined(weights);
+    // the rows are kept only for the weights' gradient
+    ctx->save_for_backward({w.defined() && w.requires_grad() ? R : at::Tensor(), w, slot, offsets});
+    return combine_rows(R, weights, slot, &offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list v = ctx->get_saved_variables();
+    const bool rows = ctx->needs_input_grad(0), weights = v[0].defined() && ctx->needs_input_grad(1);
+    variable_list out(4);
+    if (!rows && !weights) return out;
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [DR, DW] = moe_combine_backward(grads[0], or_none(v[0]), or_none(v[1]), v[2], v[3], rows, weights);
+    if (rows) out[0] = DR;
+    if (weights) out[1] = DW;
+    return once("moe_combine", std::move(out));
+  }
+};
+
+at::Tensor moe_combine(at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot, at::Tensor offsets) {
+  const at::Tensor w = or_undefined(weights);
+  return records(R, w) ? CombineFunction::apply(R, or_none(w), slot, offsets) : combine_rows(R, weights, slot, &offsets);
 }
 
 // (Q int8, S fp32 [rows]) of X [rows, dim].

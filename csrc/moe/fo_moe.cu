@@ -188,125 +188,156 @@ __device__ __forceinline__ float weight_at(const void* w, bool f32, int64_t i) {
   }
 }
 
-constexpr int kUnrollK = 8;  // rows of a token in flight per thread
+// The kernels that read a token's rows have a build for each number of rows that a thread requests at once; more choices
+// than that are taken in turns.
+constexpr int kMostAtOnce = 8;
 
-// Bound by the rows read.  A thread sums one vector of a token over its top_k rows, in their order.
 template <bool BF16>
+__device__ __forceinline__ void unpack8(const uint4& p, float2 (&f)[4]) {
+  f[0] = unpack2<BF16>(p.x);
+  f[1] = unpack2<BF16>(p.y);
+  f[2] = unpack2<BF16>(p.z);
+  f[3] = unpack2<BF16>(p.w);
+}
+
+// Bound by the rows read.  A thread sums VPT vectors of a token over its top_k rows, in their order; KC rows of them are in flight at
+// once, and where a token has few rows more of its vectors are.
+template <bool BF16, int KC, int VPT>
 __global__ void __launch_bounds__(kRowThreads)
     moe_combine_kernel(const uint4* __restrict__ R, const void* __restrict__ w, bool f32,
                        const int32_t* __restrict__ slot, uint4* __restrict__ O, int tokens, int top_k, int nvec) {
-  const int64_t v = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+  const int groups = (nvec + VPT - 1) / VPT;  // threads of a token: thread j takes vectors j, j + groups, ...
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+  const int64_t token = id / groups;
+  const int j = static_cast<int>(id - token * groups);
+  const int64_t rows = static_cast<int64_t>(tokens) * top_k;
   ptx::grid_launch_dependents();
   ptx::grid_wait();
-  const int64_t token = v / nvec;
   if (token >= tokens) return;
-  const int j = static_cast<int>(v - token * nvec);
-  const int64_t rows = static_cast<int64_t>(tokens) * top_k;
-  float acc[8];
+  float2 acc[VPT][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-  for (int k0 = 0; k0 < top_k; k0 += kUnrollK) {
-    uint4 r[kUnrollK];
-    int row[kUnrollK];
+  for (int i = 0; i < VPT; ++i) {
 #pragma unroll
-    for (int k = 0; k < kUnrollK; ++k) row[k] = k0 + k < top_k ? row_at(slot, token * top_k + k0 + k, rows) : -1;
+    for (int k = 0; k < 4; ++k) acc[i][k] = make_float2(0.f, 0.f);
+  }
+  for (int k0 = 0; k0 < top_k; k0 += KC) {
+    uint4 r[KC][VPT];
+    int row[KC];
 #pragma unroll
-    for (int k = 0; k < kUnrollK; ++k) {
-      if (row[k] >= 0) r[k] = __ldcs(R + static_cast<int64_t>(row[k]) * nvec + j);
+    for (int k = 0; k < KC; ++k) row[k] = k0 + k < top_k ? row_at(slot, token * top_k + k0 + k, rows) : -1;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (row[k] >= 0 && j + i * groups < nvec) r[k][i] = __ldcs(R + static_cast<int64_t>(row[k]) * nvec + j + i * groups);
+      }
     }
 #pragma unroll
-    for (int k = 0; k < kUnrollK; ++k) {
+    for (int k = 0; k < KC; ++k) {
       if (row[k] >= 0) {
         const float wk = weight_at<BF16>(w, f32, token * top_k + k0 + k);
-        const uint32_t u[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack2<BF16>(u[i]);
-          acc[2 * i] += wk * f.x;
-          acc[2 * i + 1] += wk * f.y;
+        for (int i = 0; i < VPT; ++i) {
+          if (j + i * groups >= nvec) continue;
+          float2 f[4];
+          unpack8<BF16>(r[k][i], f);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            acc[i][n].x += wk * f[n].x;
+            acc[i][n].y += wk * f[n].y;
+          }
         }
       }
     }
   }
-  O[v] = make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]),
-                    pack2<BF16>(acc[6], acc[7]));
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (j + i * groups < nvec) {
+      __stcs(O + token * nvec + j + i * groups,
+             make_uint4(pack2<BF16>(acc[i][0].x, acc[i][0].y), pack2<BF16>(acc[i][1].x, acc[i][1].y),
+                        pack2<BF16>(acc[i][2].x, acc[i][2].y), pack2<BF16>(acc[i][3].x, acc[i][3].y)));
+    }
+  }
 }
 
 // Bound by memory: the token's gradient is read once, every row of the experts is read (for its weight's gradient) and its
 // gradient written.  A CTA takes a token; the dots are summed over its threads in a fixed order.
-template <bool BF16, bool ROWS, bool WEIGHTS>
+template <bool BF16, int KC, int VPT, bool ROWS, bool WEIGHTS>
 __global__ void __launch_bounds__(kRowThreads)
     moe_combine_backward_kernel(const uint4* __restrict__ GO, const uint4* __restrict__ R, const void* __restrict__ w,
                                 bool f32, const int32_t* __restrict__ slot, const int32_t* __restrict__ offsets,
                                 uint4* __restrict__ DR, void* __restrict__ DW, int tokens, int top_k, int nvec,
                                 int experts) {
-  __shared__ float part[kRowThreads / 32][kUnrollK];
+  __shared__ float part[kRowThreads / 32][KC];
   const int64_t token = blockIdx.x;
   const int64_t rows = static_cast<int64_t>(tokens) * top_k;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::grid_launch_dependents();
   ptx::grid_wait();
-  for (int k0 = 0; k0 < top_k; k0 += kUnrollK) {
-    int row[kUnrollK];
-    float wk[kUnrollK], dot[kUnrollK];
+  for (int k0 = 0; k0 < top_k; k0 += KC) {
+    int row[KC];
+    float wk[KC], dot[KC];
 #pragma unroll
-    for (int k = 0; k < kUnrollK; ++k) {
+    for (int k = 0; k < KC; ++k) {
       row[k] = k0 + k < top_k ? row_at(slot, token * top_k + k0 + k, rows) : -1;
       dot[k] = 0.f;
       wk[k] = ROWS && row[k] >= 0 ? weight_at<BF16>(w, f32, token * top_k + k0 + k) : 0.f;
     }
-    for (int j = threadIdx.x; j < nvec; j += blockDim.x) {
-      const uint4 g = __ldg(GO + token * nvec + j);
-      uint4 r[kUnrollK];
+    for (int j0 = threadIdx.x; j0 < nvec; j0 += VPT * blockDim.x) {
+      uint4 g[VPT];
+      [[maybe_unused]] uint4 r[KC][VPT];
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = j0 + i * blockDim.x;
+        if (j < nvec) g[i] = __ldg(GO + token * nvec + j);
+      }
       if constexpr (WEIGHTS) {
 #pragma unroll
-        for (int k = 0; k < kUnrollK; ++k) {
-          if (row[k] >= 0) r[k] = __ldcs(R + static_cast<int64_t>(row[k]) * nvec + j);
-        }
-      }
-      const uint32_t gu[4] = {g.x, g.y, g.z, g.w};
-      float gf[8];
+        for (int k = 0; k < KC; ++k) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<BF16>(gu[i]);
-        gf[2 * i] = f.x;
-        gf[2 * i + 1] = f.y;
-      }
-#pragma unroll
-      for (int k = 0; k < kUnrollK; ++k) {
-        if (row[k] < 0) continue;
-        if constexpr (WEIGHTS) {
-          const uint32_t u[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack2<BF16>(u[i]);
-            dot[k] += gf[2 * i] * f.x + gf[2 * i + 1] * f.y;
+          for (int i = 0; i < VPT; ++i) {
+            const int j = j0 + i * blockDim.x;
+            if (row[k] >= 0 && j < nvec) r[k][i] = __ldcs(R + static_cast<int64_t>(row[k]) * nvec + j);
           }
         }
-        if constexpr (ROWS) {
-          uint4 d;
-          d.x = pack2<BF16>(wk[k] * gf[0], wk[k] * gf[1]);
-          d.y = pack2<BF16>(wk[k] * gf[2], wk[k] * gf[3]);
-          d.z = pack2<BF16>(wk[k] * gf[4], wk[k] * gf[5]);
-          d.w = pack2<BF16>(wk[k] * gf[6], wk[k] * gf[7]);
-          __stcs(DR + static_cast<int64_t>(row[k]) * nvec + j, d);
+      }
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = j0 + i * blockDim.x;
+        if (j >= nvec) continue;
+        float2 gf[4];
+        unpack8<BF16>(g[i], gf);
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+          if (row[k] < 0) continue;
+          if constexpr (WEIGHTS) {
+            float2 f[4];
+            unpack8<BF16>(r[k][i], f);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) dot[k] += gf[n].x * f[n].x + gf[n].y * f[n].y;
+          }
+          if constexpr (ROWS) {
+            __stcs(DR + static_cast<int64_t>(row[k]) * nvec + j,
+                   make_uint4(pack2<BF16>(wk[k] * gf[0].x, wk[k] * gf[0].y), pack2<BF16>(wk[k] * gf[1].x, wk[k] * gf[1].y),
+                              pack2<BF16>(wk[k] * gf[2].x, wk[k] * gf[2].y), pack2<BF16>(wk[k] * gf[3].x, wk[k] * gf[3].y)));
+          }
         }
       }
     }
     if constexpr (WEIGHTS) {
 #pragma unroll
-      for (int k = 0; k < kUnrollK; ++k) {
+      for (int k = 0; k < KC; ++k) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
       }
       __syncthreads();  // the previous round's sums have been read
       if (lane == 0) {
 #pragma unroll
-        for (int k = 0; k < kUnrollK; ++k) part[warp][k] = dot[k];
+        for (int k = 0; k < KC; ++k) part[warp][k] = dot[k];
       }
       __syncthreads();
       const int k = threadIdx.x;
-      if (k < kUnrollK && k0 + k < top_k) {
+      if (k < KC && k0 + k < top_k) {
         float s = 0.f;
         for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) s += part[i][k];
         const int64_t at = token * top_k + k0 + k;
@@ -320,7 +351,7 @@ __global__ void __launch_bounds__(kRowThreads)
       }
     }
   }
-  if constexpr (ROWS) zero_rows(DR, offsets[experts], static_cast<int64_t>(tokens) * top_k, nvec);
+  if constexpr (ROWS) zero_rows(DR, offsets[experts], rows, nvec);
 }
 
 template <typename Kernel, typename... Args>
@@ -381,15 +412,59 @@ bool valid(const MoeShape& s) {
 
 int64_t vec_ctas(const MoeShape& s) { return (static_cast<int64_t>(s.tokens) * (s.dim / 8) + kRowThreads - 1) / kRowThreads; }
 
-template <bool BF16>
-cudaError_t launch_backward(const MoeShape& s, const uint4* go, const uint4* r, MoeWeights w, const int32_t* slot,
-                            const int32_t* offsets, uint4* dr, void* dw, cudaStream_t stream) {
+// Rows requested at once, and vectors of each, for a number of choices: about eight loads a thread.
+template <bool BF16, int KC, int VPT>
+cudaError_t launch_combine(const MoeShape& s, const uint4* r, MoeWeights w, const int32_t* slot, uint4* o, cudaStream_t stream) {
   const int nvec = s.dim / 8;
-  const int threads = std::min(kRowThreads, (nvec + 31) / 32 * 32);
-  auto kernel = dr == nullptr ? moe_combine_backward_kernel<BF16, false, true>
-                : dw == nullptr ? moe_combine_backward_kernel<BF16, true, false>
-                                : moe_combine_backward_kernel<BF16, true, true>;
-  return launch(kernel, s.tokens, threads, stream, go, r, w.p, w.f32, slot, offsets, dr, dw, s.tokens, s.top_k, nvec, s.experts);
+  const int64_t threads = static_cast<int64_t>(s.tokens) * ((nvec + VPT - 1) / VPT);
+  return launch(moe_combine_kernel<BF16, KC, VPT>, (threads + kRowThreads - 1) / kRowThreads, kRowThreads, stream, r, w.p,
+                w.f32, slot, o, s.tokens, s.top_k, nvec);
+}
+
+template <bool BF16>
+cudaError_t combine(const MoeShape& s, const uint4* r, MoeWeights w, const int32_t* slot, uint4* o, cudaStream_t stream) {
+  switch (s.top_k) {
+    case 1: return launch_combine<BF16, 1, 4>(s, r, w, slot, o, stream);
+    case 2: return launch_combine<BF16, 2, 4>(s, r, w, slot, o, stream);
+    case 3: return launch_combine<BF16, 3, 2>(s, r, w, slot, o, stream);
+    case 4: return launch_combine<BF16, 4, 2>(s, r, w, slot, o, stream);
+    case 5:
+    case 6: return launch_combine<BF16, 6, 1>(s, r, w, slot, o, stream);
+    default: return launch_combine<BF16, kMostAtOnce, 1>(s, r, w, slot, o, stream);
+  }
+}
+
+struct BackwardCall {
+  MoeShape s;
+  const uint4 *go, *r;
+  MoeWeights w;
+  const int32_t *slot, *offsets;
+  uint4* dr;
+  void* dw;
+};
+
+template <bool BF16, int KC, int VPT>
+cudaError_t launch_backward(const BackwardCall& c, cudaStream_t stream) {
+  const int nvec = c.s.dim / 8;
+  const int threads = std::min(kRowThreads, ((nvec + VPT - 1) / VPT + 31) / 32 * 32);
+  auto kernel = c.dr == nullptr   ? moe_combine_backward_kernel<BF16, KC, VPT, false, true>
+                : c.dw == nullptr ? moe_combine_backward_kernel<BF16, KC, VPT, true, false>
+                                  : moe_combine_backward_kernel<BF16, KC, VPT, true, true>;
+  return launch(kernel, c.s.tokens, threads, stream, c.go, c.r, c.w.p, c.w.f32, c.slot, c.offsets, c.dr, c.dw, c.s.tokens,
+                c.s.top_k, nvec, c.s.experts);
+}
+
+template <bool BF16>
+cudaError_t backward(const BackwardCall& c, cudaStream_t stream) {
+  switch (c.s.top_k) {
+    case 1: return launch_backward<BF16, 1, 4>(c, stream);
+    case 2: return launch_backward<BF16, 2, 4>(c, stream);
+    case 3: return launch_backward<BF16, 3, 2>(c, stream);
+    case 4: return launch_backward<BF16, 4, 2>(c, stream);
+    case 5:
+    case 6: return launch_backward<BF16, 6, 1>(c, stream);
+    default: return launch_backward<BF16, kMostAtOnce, 1>(c, stream);
+  }
 }
 
 }  // namespace
@@ -411,18 +486,16 @@ cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t*
 cudaError_t moe_combine_launch(const MoeShape& s, const void* R, MoeWeights w, const int32_t* slot, void* O,
                                cudaStream_t stream) {
   if (!valid(s)) return cudaErrorInvalidValue;
-  return launch(s.bf16 ? moe_combine_kernel<true> : moe_combine_kernel<false>, vec_ctas(s), kRowThreads, stream,
-                static_cast<const uint4*>(R), w.p, w.f32, slot, static_cast<uint4*>(O), s.tokens, s.top_k, s.dim / 8);
+  const uint4* r = static_cast<const uint4*>(R);
+  return s.bf16 ? combine<true>(s, r, w, slot, static_cast<uint4*>(O), stream) : combine<false>(s, r, w, slot, static_cast<uint4*>(O), stream);
 }
 
 cudaError_t moe_combine_backward_launch(const MoeShape& s, const void* GO, const void* R, MoeWeights w,
                                         const int32_t* slot, const int32_t* offsets, void* DR, void* DW,
                                         cudaStream_t stream) {
   if (!valid(s) || (DR == nullptr && DW == nullptr)) return cudaErrorInvalidValue;
-  const uint4 *go = static_cast<const uint4*>(GO), *r = static_cast<const uint4*>(R);
-  uint4* dr = static_cast<uint4*>(DR);
-  return s.bf16 ? launch_backward<true>(s, go, r, w, slot, offsets, dr, DW, stream)
-                : launch_backward<false>(s, go, r, w, slot, offsets, dr, DW, stream);
+  const BackwardCall c{s, static_cast<const uint4*>(GO), static_cast<const uint4*>(R), w, slot, offsets, static_cast<uint4*>(DR), DW};
+  return s.bf16 ? backward<true>(c, stream) : backward<false>(c, stream);
 }
 
 }  // namespace fo

@@ -17,10 +17,9 @@ struct NormBlock {
 // stats may be nullptr.
 cudaError_t norm_block_launch(const NormBlock& p, void* H, void* Y, float* stats, int sm_count, cudaStream_t stream);
 
-// How the rows are dealt out in the backward pass: `chunks` runs of rows for every line of the gate (1 without a
-// gate, or with one line: the CTAs' own runs), `ctas` CTAs.
+// The backward pass: the CTAs that share the rows, or the clusters where a row takes one, and the scratch for their sums.
 struct NormBlockPlan {
-  int ctas, chunks;
+  int at_once;
   size_t workspace;  // floats
 };
 NormBlockPlan norm_block_plan(const NormBlock& p, int sm_count);

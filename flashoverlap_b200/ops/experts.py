@@ -2,16 +2,15 @@
 
 ``moe_sort`` turns the router's choices into an order, ``moe_dispatch`` brings the tokens' rows into it (the form
 ``OverlapImpl.gemm_all2all`` and the products by expert take), ``moe_combine`` sums the experts' rows back
-into their tokens with the router's weights.  Without a gradient to record the calls go straight to the kernels.
+into their tokens with the router's weights.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .._build import load as _load
+from ._native import native
 
 
 class ExpertOrder(NamedTuple):
@@ -21,56 +20,19 @@ class ExpertOrder(NamedTuple):
     offsets: torch.Tensor   # [experts + 1] int32: every expert's first row; the last entry is the number of rows
 
 
-def _op():
-    _load()
-    return torch.ops.flashoverlap_op
-
-
 def moe_sort(ids: torch.Tensor, experts: int) -> ExpertOrder:
     """The order of the choices ``ids`` [tokens, top_k] (int32 or int64) by expert.
 
     An id outside ``[0, experts)`` is a choice that this GPU does not serve (another rank's expert, padding): it gets no
     row.  A token may choose an expert twice.  At most 1024 experts and 64 choices a token."""
-    return ExpertOrder(*_op().moe_sort(ids, experts))
-
-
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, slot, offsets):
-        ctx.save_for_backward(slot)
-        return _op().moe_dispatch(x, slot, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        slot, = ctx.saved_tensors
-        return _op().moe_combine(g, None, slot), None, None
+    return ExpertOrder(*native("moe_sort")(ids, experts))
 
 
 def moe_dispatch(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """The rows of ``x`` [tokens, dim] in the order: [tokens * top_k, dim], rows behind the last choice zero.
 
     bf16 or fp16, ``dim`` a multiple of 8.  The gradient of a token is the fp32 sum of its rows', rounded once."""
-    slot, _, offsets = order
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Dispatch.apply(x, slot, offsets)
-    return _op().moe_dispatch(x, slot, offsets)
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, slot, offsets):
-        of_weights = weights is not None and ctx.needs_input_grad[1]
-        ctx.save_for_backward(y if of_weights else None, weights, slot, offsets)
-        return _op().moe_combine(y, weights, slot)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        y, weights, slot, offsets = ctx.saved_tensors
-        of_rows, of_weights = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        dy, dw = _op().moe_combine_backward(g, y, weights, slot, offsets, of_rows, of_weights)
-        return dy if of_rows else None, dw if of_weights else None, None, None
+    return native("moe_dispatch")(x, order[0], order[2])
 
 
 def moe_combine(y: torch.Tensor, weights: Optional[torch.Tensor], order: ExpertOrder) -> torch.Tensor:
@@ -79,7 +41,4 @@ def moe_combine(y: torch.Tensor, weights: Optional[torch.Tensor], order: ExpertO
     ``y`` [tokens * top_k, dim] in bf16 or fp16, ``dim`` a multiple of 8; ``weights`` [tokens, top_k] in fp32 or ``y``'s
     type, or None for 1.  Sums are fp32, in the order of the choices, rounded once.  The gradient of a row without a choice
     and of a weight without a row is zero."""
-    slot, _, offsets = order
-    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
-        return _Combine.apply(y, weights, slot, offsets)
-    return _op().moe_combine(y, weights, slot)
+    return native("moe_combine")(y, weights, order[0], order[2])

@@ -5,7 +5,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .._build import load as _load
+from ._native import native
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -16,8 +16,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     what is computed from it is NaN."""
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("quantize_rows has no gradient: detach its input")
-    _load()
-    return torch.ops.flashoverlap_op.quantize_rows(x)
+    return native("quantize_rows")(x)
 
 
 def linear_i8(impl, x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
