@@ -17,7 +17,8 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortCluster = 8;
+// Choices up to which one CTA sorts, and from which on sixteen do and `source` is written by all SMs; between them eight.
+constexpr int kSortOne = 4096, kSortMany = 32768;
 
 __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {
   uint32_t v;
@@ -25,11 +26,12 @@ __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr)
   return v;
 }
 
-// A stable counting sort in one launch: one CTA, or a cluster of eight.  Every warp takes a run of choices: it counts
-// them by expert in a row of its own in shared memory (lanes with equal experts find each other by
-// match.any), the counts of the warps and, through distributed shared memory, of the CTAs in front of it give
-// each warp its first row for every expert, and a second walk over the same run hands the rows out.
-// Bound by latency: the walks are chains of shared-memory updates, 32 choices a step.
+// A stable counting sort: one CTA, or a cluster of eight or sixteen.  Every warp takes a run of choices and counts them by
+// expert in a row of its own in shared memory; the counts of the warps and, through distributed shared memory, of the CTAs in
+// front of it give each warp its first row for every expert, and a second walk over the same run hands the rows out, 32
+// choices a step: ballots over the expert's bits tell each lane which others have its expert (half the time of match.any, whose
+// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us).  Bound by latency, and for many
+// choices by the scattered stores of `source`, which then all SMs do in a launch of their own.
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     moe_sort_kernel(const Id* __restrict__ ids, int64_t n, int experts, int32_t* __restrict__ slot,
@@ -59,9 +61,7 @@ __global__ void __launch_bounds__(kSortThreads)
   for (int64_t i = begin; i < end; i += 32) {
     const int e = next;
     next = expert_at(i + 32 + lane);
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    if (e < experts && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+    if (e < experts) atomicAdd(mine + e, 1u);  // a count does not depend on the order
   }
   __syncthreads();
   const int e = threadIdx.x;  // experts <= kSortThreads
@@ -114,26 +114,46 @@ __global__ void __launch_bounds__(kSortThreads)
   }
   if (rank == 0 && threadIdx.x == 0) offsets[experts] = static_cast<int32_t>(rows);
   __syncthreads();
+  const int bits = 32 - __clz(experts);
   next = expert_at(begin + lane);
   for (int64_t i = begin; i < end; i += 32) {
     const int ex = next;
     next = expert_at(i + 32 + lane);
-    const uint32_t same = __match_any_sync(0xffffffffu, ex);
+    uint32_t same = 0xffffffffu;  // the lanes with this lane's expert
+    for (int b = 0; b < bits; ++b) {
+      const uint32_t ones = __ballot_sync(0xffffffffu, (ex >> b) & 1);
+      same &= (ex >> b) & 1 ? ones : ~ones;
+    }
     int32_t row = -1;
     if (ex < experts) {
       row = static_cast<int32_t>(mine[ex] + __popc(same & ((1u << lane) - 1u)));
-      source[row] = static_cast<int32_t>(i + lane);
+      if (source != nullptr) source[row] = static_cast<int32_t>(i + lane);
     }
     __syncwarp();
     if (ex < experts && lane == __ffs(same) - 1) mine[ex] += __popc(same);
     __syncwarp();
     if (i + lane < end) slot[i + lane] = row;
   }
-  for (int64_t r = rows + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n; r += static_cast<int64_t>(ctas) * kSortThreads) {
-    source[r] = -1;
+  if (source != nullptr) {
+    for (int64_t r = rows + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n; r += static_cast<int64_t>(ctas) * kSortThreads) {
+      source[r] = -1;
+    }
   }
   __syncwarp();
   ptx::cluster_wait_acquire();
+}
+
+// source[slot[i]] = i, and -1 behind the last row.
+__global__ void __launch_bounds__(256)
+    moe_source_kernel(const int32_t* __restrict__ slot, const int32_t* __restrict__ offsets, int32_t* __restrict__ source,
+                      int n, int experts) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+  if (i >= n) return;
+  const int row = slot[i];
+  if (row >= 0) source[row] = static_cast<int32_t>(i);
+  if (i >= offsets[experts]) source[i] = -1;
 }
 
 // ---------------------------------------------------------------------------- the rows
@@ -380,12 +400,14 @@ cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, 
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (kSortWarps + 1) * kMaxExperts * static_cast<int>(sizeof(uint32_t)));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (kSortWarps + 1) * kMaxExperts * static_cast<int>(sizeof(uint32_t)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 16) set[dev] = true;
   }
-  const int ctas = n <= 4 * kSortThreads ? 1 : kSortCluster;
+  const bool many = n > kSortMany;
+  const int ctas = n <= kSortOne ? 1 : (many ? 16 : 8);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -400,9 +422,11 @@ cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), n, experts, slot, source, offsets);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), n, experts, slot, many ? nullptr : source, offsets);
   if (e != cudaSuccess) cudaGetLastError();
-  return e;
+  if (e != cudaSuccess || !many) return e;
+  return launch(moe_source_kernel, (n + 255) / 256, 256, stream, static_cast<const int32_t*>(slot), static_cast<const int32_t*>(offsets),
+                source, static_cast<int>(n), experts);
 }
 
 bool valid(const MoeShape& s) {
