@@ -30,6 +30,7 @@ struct GemmI8Params {
 
 struct GemmI8Maps {
   CUtensorMap a, b, c;
+  CUtensorMap b_half;  // wide kernel: boxes of half of b's rows, for half-width tiles
 };
 
 // What runs for a problem: the wide kernel (256 x 256 tiles, CTA pairs), or the narrow one (tiles of `tokens` tokens x 128

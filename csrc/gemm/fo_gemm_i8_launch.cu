@@ -4,6 +4,7 @@
 #include "fo_gemm_i8_sm100.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace fo {
 
@@ -69,7 +70,8 @@ cudaError_t launch_wide(const GemmI8Maps& maps, const GemmI8Params& p, cudaStrea
   if (e != cudaSuccess) return e;
   // with offsets, every expert may end in a tile of its own
   const int64_t units = ((p.M + kI8Rows - 1) / kI8Rows + (GROUPED ? std::min(p.experts, p.M) : 0)) * static_cast<int64_t>(p.tiles_n);
-  const int64_t pairs = std::min<int64_t>(units, resident_pairs<BF16, GROUPED>());
+  const int64_t resident = resident_pairs<BF16, GROUPED>();
+  const int64_t pairs = GROUPED || 2 * units <= resident ? std::min(2 * units, resident) : std::min(units, resident);
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = config(2 * pairs, kI8WideThreads, smem, 2, stream, attr);
   return cudaLaunchKernelEx(&cfg, kernel, maps, p);
@@ -118,15 +120,71 @@ cudaError_t dispatch(const GemmI8Plan& plan, const GemmI8Maps& maps, const GemmI
 
 }  // namespace
 
+// ---------------------------------------------------------------------------- choice of a kernel
+//
+// A model of the time of one call, in us, with what was measured on a B200 (cold, less 8 us that an empty call reads):
+//  * the wide kernel's pairs take 0.34 us a k-block of 128 for a 256 x 256 tile (3.7 PFLOP/s), 0.23 us for a half, and 2.5 us at
+//    the end of a wave; 256 x 8192 x 28672: 51 us in halves, 1024 x 28672 x 8192: 133 us.  Its loads reach 5.9 TB/s;
+//  * a narrow kernel's SM takes in 140 KB/us, a CTA with half an SM's memory 92 at most, all together 6.3 TB/s of weights; the epilogue
+//    takes 0.045 us a token (64 tokens x 1024 deep: 2.8 us of products, 2.9 us of stores), the exchange of a split 0.7 us and 26 KB/us.
+// The two sides for one token x 8192 x 28672: 94 us wide, 34 us as 16 tokens split in four; 128 x 8192 x 28672: 51 and 41;
+// 256 x 28672 x 8192: 47 and 80; 192 x 1024 x 8192: 14 and 6; 4096 rows of 64 experts x 3584 x 4096: 162 and 188, 512 rows: 137 and 125.
+namespace {
+
+constexpr int kPairs = 74;
+
+// Weight matrices that are used, and the tiles of `rows` tokens that each has: about half of a tile is empty at an expert's end.
+struct I8Load {
+  double matrices, tiles_each;
+};
+I8Load i8_load(int M, int experts, bool grouped, int rows) {
+  if (!grouped) return I8Load{1.0, static_cast<double>((M + rows - 1) / rows)};
+  const double used = std::min(experts, M);
+  return I8Load{used, std::max(1.0, M / used / rows + 0.5)};
+}
+
+double wide_time(int M, int N, int K, int experts, bool grouped) {
+  const double num_kb = (K + kI8BK - 1) / kI8BK;
+  const I8Load l = i8_load(M, experts, grouped, kI8Rows);
+  const int64_t units = static_cast<int64_t>(l.matrices * l.tiles_each + 0.5) * ((N + kI8Cols - 1) / kI8Cols);
+  const int64_t left = units % kPairs;
+  const double last = left == 0 ? 0.0 : (2 * left <= kPairs ? 0.23 : 0.34) * num_kb;
+  const double weights = 1e-6 * l.matrices * N * K / 5.9;
+  return std::max(units / kPairs * 0.34 * num_kb + last, weights) + 2.5;
+}
+
+double narrow_time(int M, int N, int K, int experts, bool grouped, int tokens, int split) {
+  const int num_kb = ((K + kI8BK - 1) / kI8BK + split - 1) / split;
+  const I8Load l = i8_load(M, experts, grouped, tokens);
+  const double ctas = l.matrices * l.tiles_each * ((N + 127) / 128) * split;
+  const int slots = tokens == 128 ? 2 * kPairs : 4 * kPairs;
+  auto wave = [&](double n) {
+    const double rate = n > 2 * kPairs ? 140e3 * 2 * kPairs / slots : (tokens == 128 ? 140e3 : 92e3);
+    const double loads = num_kb * (16384.0 + 128.0 * tokens) / rate;
+    const double weights = n / l.tiles_each * num_kb * 16384.0 / 6.3e6;
+    return std::max(loads, weights) + 0.045 * tokens / split;
+  };
+  const double full = std::floor(ctas / slots), rest = ctas - full * slots;
+  const double exchange = split > 1 ? 0.7 + tokens * 512.0 * (split - 1) / split / 26e3 : 0.0;
+  if (split > 1 && ctas > slots) return 1e30;  // clusters in a second wave wait for room for all of their CTAs
+  return full * wave(slots) + (rest > 0 ? wave(rest) : 0.0) + exchange;
+}
+
+}  // namespace
+
 GemmI8Plan choose_i8(int M, int N, int K, int experts, bool grouped) {
   GemmI8Plan plan{0, 1};
-  const int per = grouped ? (M + experts - 1) / experts : M;  // tokens of a weight matrix
-  if (per > 128) return plan;
-  plan.tokens = per <= 16 ? 16 : per <= 32 ? 32 : per <= 64 ? 64 : 128;
-  const int64_t tiles = static_cast<int64_t>((N + 127) / 128) * (grouped ? std::min(experts, M) : 1);
-  const int num_kb = (K + kI8BK - 1) / kI8BK;
-  const int slots = plan.tokens == 128 ? 148 : 296;
-  while (plan.split < 8 && plan.split * 2 * 4 <= plan.tokens && tiles * plan.split * 2 <= slots && num_kb >= plan.split * 4) plan.split *= 2;
+  double best = wide_time(M, N, K, experts, grouped);
+  for (int tokens : {16, 32, 64, 128}) {
+    for (int split : {1, 2, 4, 8}) {
+      if (4 * split > tokens || split * kI8BK > K) continue;  // sums are exchanged four tokens at a time
+      const double t = narrow_time(M, N, K, experts, grouped, tokens, split);
+      if (t < best) {
+        best = t;
+        plan = GemmI8Plan{tokens, split};
+      }
+    }
+  }
   return plan;
 }
 
@@ -137,6 +195,8 @@ std::string gemm_i8_launch(const GemmI8Plan& plan, GemmI8Params p, const void* A
   std::string e = encode_tmap_8bit(&maps.a, A, 1, p.M, p.K, wide ? 128 : plan.tokens, false);
   if (!e.empty()) return "A: " + e;
   e = encode_tmap_8bit(&maps.b, B, p.experts, p.N, p.K, 128, true);
+  if (!e.empty()) return "B: " + e;
+  e = encode_tmap_8bit(&maps.b_half, B, p.experts, p.N, p.K, 64, true);
   if (!e.empty()) return "B: " + e;
   e = encode_tmap_16bit(&maps.c, p.C, p.M, p.N, 32);
   if (!e.empty()) return "C: " + e;

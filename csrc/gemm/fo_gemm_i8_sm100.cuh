@@ -155,16 +155,23 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
     __syncthreads();
     units_m = s_first[p.experts];
   }
-  const int sched_len = units_m * p.tiles_n;
+  // The tiles that are left over after the last full wave are computed as 256 x 128 halves if those fit one wave.
+  const int sched_tiles = units_m * p.tiles_n;
+  const int left = sched_tiles % num_units;
+  const int tail_start = sched_tiles - (2 * left <= num_units ? left : 0);
+  const int sched_len = 2 * sched_tiles - tail_start;
 
   struct Work {
     int row, row_end;  // this CTA's first row, and the end of the rows that are stored
     int n0, expert;
+    bool narrow;  // 128 columns from n0
   };
-  auto work_at = [&](int pos) {
-    const TileCoord tc = tile_of_position(pos, units_m, p.tiles_n, p.raster_sw);
+  auto work_at = [&](int i) {
     Work w;
-    w.n0 = tc.n * kI8Cols;
+    w.narrow = i >= tail_start;
+    const int pos = w.narrow ? tail_start + (i - tail_start) / 2 : i;
+    const TileCoord tc = tile_of_position(pos, units_m, p.tiles_n, p.raster_sw);
+    w.n0 = tc.n * kI8Cols + (w.narrow ? ((i - tail_start) & 1) * (kI8Cols / 2) : 0);
     if constexpr (GROUPED) {
       int lo = 0, hi = p.experts;  // the last expert whose first unit is not behind tc.m has it
       while (hi - lo > 1) {
@@ -205,10 +212,12 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
         if (elected) {
           uint8_t* sa = smem + stage * L::kStageBytes;
           // the leader's barrier collects the bytes of both CTAs
-          if (leader) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kStageBytes);
+          if (leader) {
+            ptx::mbar_arrive_expect_tx(&full_bar[stage], 2 * (work.narrow ? L::kStageBytes - L::kBBytes / 2 : L::kStageBytes));
+          }
           ptx::tma_load_2d_pair(sa, &maps.a, &full_bar[stage], kb * kI8BK, work.row, ptx::kL2EvictNormal);
-          ptx::tma_load_3d_pair(sa + L::kABytes, &maps.b, &full_bar[stage], kb * kI8BK, work.n0 + rank * 128,
-                                work.expert, ptx::kL2EvictNormal);
+          ptx::tma_load_3d_pair(sa + L::kABytes, work.narrow ? &maps.b_half : &maps.b, &full_bar[stage], kb * kI8BK,
+                                work.n0 + rank * (work.narrow ? 64 : 128), work.expert, ptx::kL2EvictNormal);
         }
         __syncwarp();
         ++issued;
@@ -230,7 +239,8 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
     // ------------------------------------------------------------------ MMA issuer
     if (leader) {
       const bool elected = ptx::elect_one();
-      constexpr uint32_t idesc = ptx::make_idesc_s8(kI8Rows, kI8Cols);
+      constexpr uint32_t idesc_full = ptx::make_idesc_s8(kI8Rows, kI8Cols);
+      constexpr uint32_t idesc_half = ptx::make_idesc_s8(kI8Rows, kI8Cols / 2);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -244,6 +254,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
         }
         ptx::tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kI8Cols);
+        const uint32_t idesc = pos >= tail_start ? idesc_half : idesc_full;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!ptx::mbar_wait_bounded(&full_bar[stage], phase, s_abort, pipe_timeout)) {
             if (elected) ptx::report_status(p.status, kStatusTimeoutSmemFull, pos, kb, stage);
@@ -309,13 +320,14 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
       ptx::tc_fence_after_sync();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kI8Cols);
       const bool last_tile = pos + num_units >= sched_len;
+      const int chunks = (work.narrow ? kI8Cols / 2 : kI8Cols) / 64;
 #pragma unroll 1
-      for (int c = wg; c < kI8Cols / 64; c += 2) {
+      for (int c = wg; c < chunks; c += 2) {
         uint32_t v0[32], v1[32];
         ptx::tmem_ld_32x32b_x32(t_row + c * 64, v0);
         ptx::tmem_ld_32x32b_x32(t_row + c * 64 + 32, v1);
         ptx::tmem_ld_wait();
-        if (c + 2 >= kI8Cols / 64) {
+        if (c + 2 >= chunks) {
           // accumulator fully read by this warp: hand it back to the leader's MMA warp
           ptx::tc_fence_before_sync();
           __syncwarp();
