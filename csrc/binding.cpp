@@ -197,7 +197,7 @@ NormBlockOperands norm_block_operands(const at::Tensor& X, const at::Tensor& T, 
 }
 
 // (H, Y, stats): u = rmsnorm(T) * PW, H = alpha * X + G * u, Y = rmsnorm(H) * W; stats [rows, 2] fp32 (1 / rms of T and of H),
-// what the backward pass needs, if asked for, else empty.
+// what the backward pass needs, if asked for, else None.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_block_forward(at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
                                                                   c10::optional<at::Tensor> G, double alpha, double eps,
                                                                   bool with_stats) {
@@ -205,7 +205,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_block_forward(at::Tensor X, 
   c10::cuda::CUDAGuard guard(X.device());
   const NormBlockOperands o = norm_block_operands(X, T, PW, W, G, alpha, eps);
   at::Tensor H = at::empty(X.sizes(), o.X.options()), Y = at::empty(X.sizes(), o.X.options());
-  at::Tensor stats = at::empty({with_stats ? X.size(0) : 0, 2}, o.X.options().dtype(at::kFloat));
+  at::Tensor stats;
+  if (with_stats) stats = at::empty({X.size(0), 2}, o.X.options().dtype(at::kFloat));
   if (o.p.rows > 0) {
     fo::cuda_check(fo::norm_block_launch(o.p, H.data_ptr(), Y.data_ptr(), with_stats ? stats.data_ptr<float>() : nullptr,
                                          sm_count_of_current_device(), c10::cuda::getCurrentCUDAStream().stream()),

@@ -37,7 +37,7 @@ struct GemmI8Maps {
 // channels, K split over the `split` CTAs of a cluster).
 struct GemmI8Plan {
   int tokens;  // 0: wide
-  int split;
+  int split;   // narrow; wide: 1, or 2 for tiles of 512 rows
 };
 GemmI8Plan choose_i8(int M, int N, int K, int experts, bool grouped);
 

@@ -38,7 +38,7 @@ cudaLaunchConfig_t config(int64_t grid, int threads, int smem, int cluster, cuda
 }
 
 // CTA pairs of the wide kernel that run at once on the current device.
-template <bool BF16, bool GROUPED>
+template <bool BF16, bool GROUPED, int MT>
 int resident_pairs() {
   static int cache[16] = {};  // 0: not asked yet
   int dev = 0;
@@ -48,10 +48,10 @@ int resident_pairs() {
     int sm_count = 0, clusters = 0;
     cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev);
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = config(sm_count & ~1, kI8WideThreads, I8WideSmem<GROUPED>::kTotalBytes, 2, nullptr, attr);
+    cudaLaunchConfig_t cfg = config(sm_count & ~1, kI8WideThreads, I8WideSmem<GROUPED, MT>::kTotalBytes, 2, nullptr, attr);
     cfg.attrs = attr + 1;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&clusters, fo_gemm_i8_wide_kernel<BF16, GROUPED>, &cfg) != cudaSuccess || clusters < 1) {
+    if (cudaOccupancyMaxActiveClusters(&clusters, fo_gemm_i8_wide_kernel<BF16, GROUPED, MT>, &cfg) != cudaSuccess || clusters < 1) {
       cudaGetLastError();
       clusters = 1;
     }
@@ -60,18 +60,18 @@ int resident_pairs() {
   return cache[dev];
 }
 
-template <bool BF16, bool GROUPED>
+template <bool BF16, bool GROUPED, int MT>
 cudaError_t launch_wide(const GemmI8Maps& maps, const GemmI8Params& p, cudaStream_t stream) {
-  constexpr int smem = I8WideSmem<GROUPED>::kTotalBytes;
+  constexpr int smem = I8WideSmem<GROUPED, MT>::kTotalBytes;
   static_assert(smem <= 227 * 1024, "shared memory of this configuration exceeds 227 KB");
   static bool attr_set[16] = {};
-  auto kernel = fo_gemm_i8_wide_kernel<BF16, GROUPED>;
+  auto kernel = fo_gemm_i8_wide_kernel<BF16, GROUPED, MT>;
   const cudaError_t e = prepare(kernel, smem, attr_set);
   if (e != cudaSuccess) return e;
   // with offsets, every expert may end in a tile of its own
-  const int64_t units = ((p.M + kI8Rows - 1) / kI8Rows + (GROUPED ? std::min(p.experts, p.M) : 0)) * static_cast<int64_t>(p.tiles_n);
-  const int64_t resident = resident_pairs<BF16, GROUPED>();
-  const int64_t pairs = GROUPED || 2 * units <= resident ? std::min(2 * units, resident) : std::min(units, resident);
+  const int64_t units = ((p.M + MT * kI8Rows - 1) / (MT * kI8Rows) + (GROUPED ? std::min(p.experts, p.M) : 0)) * static_cast<int64_t>(p.tiles_n);
+  const int64_t resident = resident_pairs<BF16, GROUPED, MT>();
+  const int64_t pairs = MT == 1 && (GROUPED || 2 * units <= resident) ? std::min(2 * units, resident) : std::min(units, resident);
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = config(2 * pairs, kI8WideThreads, smem, 2, stream, attr);
   return cudaLaunchKernelEx(&cfg, kernel, maps, p);
@@ -109,7 +109,9 @@ cudaError_t dispatch_split(int split, const GemmI8Maps& maps, const GemmI8Params
 template <bool BF16>
 cudaError_t dispatch(const GemmI8Plan& plan, const GemmI8Maps& maps, const GemmI8Params& p, cudaStream_t stream) {
   switch (plan.tokens) {
-    case 0: return p.offsets != nullptr ? launch_wide<BF16, true>(maps, p, stream) : launch_wide<BF16, false>(maps, p, stream);
+    case 0:
+      if (p.offsets != nullptr) return launch_wide<BF16, true, 1>(maps, p, stream);
+      return plan.split == 2 ? launch_wide<BF16, false, 2>(maps, p, stream) : launch_wide<BF16, false, 1>(maps, p, stream);
     case 16: return dispatch_split<BF16, 16>(plan.split, maps, p, stream);
     case 32: return dispatch_split<BF16, 32>(plan.split, maps, p, stream);
     case 64: return dispatch_split<BF16, 64>(plan.split, maps, p, stream);
@@ -143,11 +145,17 @@ I8Load i8_load(int M, int experts, bool grouped, int rows) {
   return I8Load{used, std::max(1.0, M / used / rows + 0.5)};
 }
 
-double wide_time(int M, int N, int K, int experts, bool grouped) {
+// mt: 1, or 2 for tiles of 512 x 256.  Those take 0.66 us a k-block where the call is bound by power, and that is what they are for:
+// under sustained load 8192 x 8192 x 28672 takes 1303 us in them and 1365 in tiles of 256, but 8192 x 28672 x 8192 1378 and 1340,
+// 16384 x 8192 x 3584 368 and 352, 4096 x 4096 x 4096 55 and 50.
+constexpr int kTallTilesK = 16384;
+
+double wide_time(int M, int N, int K, int experts, bool grouped, int mt = 1) {
   const double num_kb = (K + kI8BK - 1) / kI8BK;
-  const I8Load l = i8_load(M, experts, grouped, kI8Rows);
+  const I8Load l = i8_load(M, experts, grouped, mt * kI8Rows);
   const int64_t units = static_cast<int64_t>(l.matrices * l.tiles_each + 0.5) * ((N + kI8Cols - 1) / kI8Cols);
   const int64_t left = units % kPairs;
+  if (mt == 2) return static_cast<double>((units + kPairs - 1) / kPairs) * (0.66 * num_kb + 3.5);
   const double last = left == 0 ? 0.0 : (2 * left <= kPairs ? 0.23 : 0.34) * num_kb;
   const double weights = 1e-6 * l.matrices * N * K / 5.9;
   return std::max(units / kPairs * 0.34 * num_kb + last, weights) + 2.5;
@@ -175,6 +183,13 @@ double narrow_time(int M, int N, int K, int experts, bool grouped, int tokens, i
 GemmI8Plan choose_i8(int M, int N, int K, int experts, bool grouped) {
   GemmI8Plan plan{0, 1};
   double best = wide_time(M, N, K, experts, grouped);
+  if (!grouped && K >= kTallTilesK) {
+    const double t = wide_time(M, N, K, experts, grouped, 2);
+    if (t < best) {
+      best = t;
+      plan = GemmI8Plan{0, 2};
+    }
+  }
   for (int tokens : {16, 32, 64, 128}) {
     for (int split : {1, 2, 4, 8}) {
       if (4 * split > tokens || split * kI8BK > K) continue;  // sums are exchanged four tokens at a time
@@ -196,10 +211,12 @@ std::string gemm_i8_launch(const GemmI8Plan& plan, GemmI8Params p, const void* A
   if (!e.empty()) return "A: " + e;
   e = encode_tmap_8bit(&maps.b, B, p.experts, p.N, p.K, 128, true);
   if (!e.empty()) return "B: " + e;
-  e = encode_tmap_8bit(&maps.b_half, B, p.experts, p.N, p.K, 64, true);
-  if (!e.empty()) return "B: " + e;
-  e = encode_tmap_16bit(&maps.c, p.C, p.M, p.N, 32);
-  if (!e.empty()) return "C: " + e;
+  if (wide) {
+    e = encode_tmap_8bit(&maps.b_half, B, p.experts, p.N, p.K, 64, true);
+    if (!e.empty()) return "B: " + e;
+    e = encode_tmap_16bit(&maps.c, p.C, p.M, p.N, 32);
+    if (!e.empty()) return "C: " + e;
+  }
   p.tiles_n = (p.N + kI8Cols - 1) / kI8Cols;
   p.raster_sw = std::min(8, p.tiles_n);
   if (!wide) {

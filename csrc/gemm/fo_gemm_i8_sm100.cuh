@@ -54,10 +54,14 @@ __device__ __forceinline__ I8Segment i8_segment(const GemmI8Params& p, int e) {
 constexpr int kI8Rows = 256, kI8Cols = 256;  // tile of a CTA pair
 constexpr int kI8WideThreads = 64 + 256;
 
-template <bool GROUPED>
+// MT = 2: each CTA of a pair owns two 128-row halves that share its B tile (512 x 256 per pair): a quarter fewer operand bytes a
+// product, but the two accumulators fill TMEM, so nothing hides a tile's epilogue.
+template <bool GROUPED, int MT>
 struct I8WideSmem {
-  static constexpr int kStages = GROUPED ? 5 : 6;  // the experts' tables take a stage's place
-  static constexpr int kABytes = 128 * kI8BK;
+  static_assert(MT == 1 || !GROUPED, "experts' rows come in 256-row tiles");
+  static constexpr int kStages = MT == 2 ? 4 : (GROUPED ? 5 : 6);  // the experts' tables take a stage's place
+  static constexpr int kAHalfBytes = 128 * kI8BK;
+  static constexpr int kABytes = MT * kAHalfBytes;
   static constexpr int kBBytes = 128 * kI8BK;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kWarpBufBytes = 32 * 128;  // 32 rows x 64 16-bit columns
@@ -70,11 +74,13 @@ struct I8WideSmem {
   static constexpr int kTotalBytes = kMiscOffset + 16 + 1024;
 };
 
-template <bool BF16, bool GROUPED>
+template <bool BF16, bool GROUPED, int MT>
 __global__ void __launch_bounds__(kI8WideThreads, 1)
     fo_gemm_i8_wide_kernel(const __grid_constant__ GemmI8Maps maps, const __grid_constant__ GemmI8Params p) {
-  using L = I8WideSmem<GROUPED>;
+  using L = I8WideSmem<GROUPED, MT>;
   constexpr int STAGES = L::kStages;
+  constexpr int kRows = MT * kI8Rows;             // of a pair's tile
+  constexpr int kAccStages = MT == 2 ? 1 : 2;     // tiles whose accumulators TMEM holds
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
@@ -128,7 +134,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
   ptx::grid_launch_dependents();
   ptx::grid_wait();
 
-  int units_m = (p.M + kI8Rows - 1) / kI8Rows;
+  int units_m = (p.M + kRows - 1) / kRows;
   if constexpr (GROUPED) {
     for (int e = threadIdx.x; e < p.experts; e += kI8WideThreads) {
       const I8Segment s = i8_segment(p, e);
@@ -158,7 +164,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
   // The tiles that are left over after the last full wave are computed as 256 x 128 halves if those fit one wave.
   const int sched_tiles = units_m * p.tiles_n;
   const int left = sched_tiles % num_units;
-  const int tail_start = sched_tiles - (2 * left <= num_units ? left : 0);
+  const int tail_start = sched_tiles - (MT == 1 && 2 * left <= num_units ? left : 0);
   const int sched_len = 2 * sched_tiles - tail_start;
 
   struct Work {
@@ -168,7 +174,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
   };
   auto work_at = [&](int i) {
     Work w;
-    w.narrow = i >= tail_start;
+    w.narrow = MT == 1 && i >= tail_start;
     const int pos = w.narrow ? tail_start + (i - tail_start) / 2 : i;
     const TileCoord tc = tile_of_position(pos, units_m, p.tiles_n, p.raster_sw);
     w.n0 = tc.n * kI8Cols + (w.narrow ? ((i - tail_start) & 1) * (kI8Cols / 2) : 0);
@@ -187,7 +193,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
       w.row_end = p.offsets[lo + 1];
     } else {
       w.expert = 0;
-      w.row = tc.m * kI8Rows + rank * 128;
+      w.row = tc.m * kRows + rank * MT * 128;
       w.row_end = p.M;
     }
     return w;
@@ -215,7 +221,11 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
           if (leader) {
             ptx::mbar_arrive_expect_tx(&full_bar[stage], 2 * (work.narrow ? L::kStageBytes - L::kBBytes / 2 : L::kStageBytes));
           }
-          ptx::tma_load_2d_pair(sa, &maps.a, &full_bar[stage], kb * kI8BK, work.row, ptx::kL2EvictNormal);
+#pragma unroll
+          for (int h = 0; h < MT; ++h) {
+            ptx::tma_load_2d_pair(sa + h * L::kAHalfBytes, &maps.a, &full_bar[stage], kb * kI8BK, work.row + h * 128,
+                                  ptx::kL2EvictNormal);
+          }
           ptx::tma_load_3d_pair(sa + L::kABytes, work.narrow ? &maps.b_half : &maps.b, &full_bar[stage], kb * kI8BK,
                                 work.n0 + rank * (work.narrow ? 64 : 128), work.expert, ptx::kL2EvictNormal);
         }
@@ -254,7 +264,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
         }
         ptx::tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kI8Cols);
-        const uint32_t idesc = pos >= tail_start ? idesc_half : idesc_full;
+        const uint32_t idesc = MT == 1 && pos >= tail_start ? idesc_half : idesc_full;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!ptx::mbar_wait_bounded(&full_bar[stage], phase, s_abort, pipe_timeout)) {
             if (elected) ptx::report_status(p.status, kStatusTimeoutSmemFull, pos, kb, stage);
@@ -269,9 +279,13 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
           if (elected) {
             // advance 32 elements (32 B) along K inside the swizzle atom: +2 in 16-byte units
 #pragma unroll
-            for (int k = 0; k < kI8BK / 32; ++k) {
-              ptx::umma_s8_ss_pair(tmem_d, da + static_cast<uint64_t>(2 * k), db + static_cast<uint64_t>(2 * k), idesc,
-                                   (kb > 0 || k > 0) ? 1u : 0u);
+            for (int h = 0; h < MT; ++h) {
+#pragma unroll
+              for (int k = 0; k < kI8BK / 32; ++k) {
+                ptx::umma_s8_ss_pair(tmem_d + static_cast<uint32_t>(h * kI8Cols),
+                                     da + static_cast<uint64_t>(h * (L::kAHalfBytes >> 4) + 2 * k),
+                                     db + static_cast<uint64_t>(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+              }
             }
             ptx::umma_commit_pair(&empty_bar[stage], 3);  // slot reusable in both CTAs
           }
@@ -284,7 +298,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
         if (!ok) break;
         if (elected) ptx::umma_commit_pair(&tmem_full_bar[acc], 3);  // accumulators complete in both CTAs
         __syncwarp();
-        if (++acc == 2) {
+        if (++acc == kAccStages) {
           acc = 0;
           acc_phase ^= 1u;
         }
@@ -293,7 +307,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
   } else {
     // ------------------------------------------------------------------ epilogue
     const int ew = warp_idx - 2;
-    const int wg = ew >> 2;         // every second 64-column chunk
+    const int wg = ew >> 2;         // every second 64-column chunk, or (MT = 2) all chunks of one half
     const int quad = warp_idx & 3;  // TMEM lane quadrant this warp may read
     uint8_t* buf = smem + L::kEpiOffset + ew * L::kWarpBufBytes;
     int acc = 0;
@@ -302,7 +316,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
     const uint32_t tmem_empty_addr0 = ptx::mapa_shared(ptx::smem_u32(&tmem_empty_bar[0]), 0u);  // the leader's
     for (int pos = unit; ok && pos < sched_len; pos += num_units) {
       const Work work = work_at(pos);
-      const int row0 = work.row + quad * 32;
+      const int row0 = work.row + (MT == 2 ? wg * 128 : 0) + quad * 32;
       const bool exists = row0 < work.row_end;
       // whole rows of the warp leave by tensor store (which leaves out what lies beyond the matrix), an expert's last
       // ones by thread, since behind them are the next expert's
@@ -318,16 +332,18 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
         break;
       }
       ptx::tc_fence_after_sync();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kI8Cols);
+      const uint32_t t_row =
+          tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>((MT == 2 ? wg : acc) * kI8Cols);
+      constexpr int kStep = MT == 2 ? 1 : 2;  // chunks a warp steps by
       const bool last_tile = pos + num_units >= sched_len;
       const int chunks = (work.narrow ? kI8Cols / 2 : kI8Cols) / 64;
 #pragma unroll 1
-      for (int c = wg; c < chunks; c += 2) {
+      for (int c = MT == 2 ? 0 : wg; c < chunks; c += kStep) {
         uint32_t v0[32], v1[32];
         ptx::tmem_ld_32x32b_x32(t_row + c * 64, v0);
         ptx::tmem_ld_32x32b_x32(t_row + c * 64 + 32, v1);
         ptx::tmem_ld_wait();
-        if (c + 2 >= chunks) {
+        if (c + kStep >= chunks) {
           // accumulator fully read by this warp: hand it back to the leader's MMA warp
           ptx::tc_fence_before_sync();
           __syncwarp();
@@ -335,11 +351,12 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
         }
         const int cols = p.N - work.n0 - c * 64;  // of the matrix, from the chunk's first on
         if (!exists || cols <= 0) continue;
-        // On the CTA's last tile the operand ring is idle: the second chunk goes through it instead of waiting for the
+        // On the CTA's last tile the operand ring is idle: the later chunks go through it instead of waiting for the
         // buffer's previous store.
+        static_assert(8 * (kI8Cols / 64) * L::kWarpBufBytes <= L::kEpiOffset, "the ring must hold a tile");
         uint8_t* cbuf = buf;
-        if (last_tile && c >= 2) {
-          cbuf = smem + ew * L::kWarpBufBytes;
+        if (last_tile && c >= kStep) {
+          cbuf = smem + (ew * (kI8Cols / 64) + c) * L::kWarpBufBytes;
         } else {
           if (lane == 0) ptx::bulk_wait_group_read<0>();
           __syncwarp();
@@ -382,7 +399,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
           __syncwarp();  // everybody has read the buffer before it is written again
         }
       }
-      if (++acc == 2) {
+      if (++acc == kAccStages) {
         acc = 0;
         acc_phase ^= 1u;
       }

@@ -11,7 +11,6 @@
 #include "../common/fo_nvtx.h"
 #include "../elementwise/fo_elementwise.h"
 #include "../flags/fo_wait.h"
-#include "../gemm/fo_gemm_i8.h"
 #include "../norm/fo_norm.h"
 #include "fused_common.h"
 
@@ -442,88 +441,106 @@ void OverlapImpl::GemmSwiGLU(at::Tensor A, at::Tensor B, at::Tensor C) {
   cuda_check(launch_gemm(kPairAlgo, s.bf16, false, maps, p, grid, 1, false, stream()), "SwiGLU GEMM launch");
 }
 
-void OverlapImpl::GemmI8(at::Tensor A, at::Tensor B, at::Tensor SA, at::Tensor SB, at::Tensor C,
-                         c10::optional<at::Tensor> offsets) {
-  NvtxRange nvtx_range("flashoverlap::gemm_i8");
-  FO_CHECK(world_ == 1, "gemm_i8 is a single-rank call");
-  FO_CHECK(A.is_cuda() && A.dim() == 2 && A.is_contiguous() && A.scalar_type() == at::kChar,
-           "A must be a contiguous int8 CUDA tensor [M, K]");
+// B and its scales of an 8-bit product, and offsets if it is by expert: checked against K and against the device of `like`.
+static void check_i8_weights(const at::Tensor& like, int64_t K, const at::Tensor& B, const at::Tensor& SB,
+                             const c10::optional<at::Tensor>& offsets, GemmI8Params* p) {
   const bool grouped = offsets.has_value() && offsets->defined();
   FO_CHECK(B.is_cuda() && B.is_contiguous() && B.scalar_type() == at::kChar && B.dim() == (grouped ? 3 : 2),
            grouped ? "B must be a contiguous int8 CUDA tensor [experts, N, K]" : "B must be a contiguous int8 CUDA tensor [N, K]");
-  const int64_t M = A.size(0), K = A.size(1), N = B.size(-2), E = grouped ? B.size(0) : 1;
-  FO_CHECK(B.size(-1) == K, "A [M, K] and B disagree on K");
+  const int64_t N = B.size(-2), E = grouped ? B.size(0) : 1;
+  FO_CHECK(B.size(-1) == K, "the activations [..., K] and B disagree on K");
   FO_CHECK(K >= 16 && K % 16 == 0 && K <= kI8MaxK, "K must be a multiple of 16 from 16 to ", kI8MaxK, " (K=", K, ")");
-  FO_CHECK(N >= 8 && N % 8 == 0 && N <= INT32_MAX && M <= INT32_MAX, "N must be a multiple of 8 (N=", N, ")");
-  FO_CHECK(SA.is_cuda() && SA.is_contiguous() && SA.scalar_type() == at::kFloat && SA.dim() == 1 && SA.size(0) == M,
-           "SA must be a contiguous float32 CUDA tensor [M]");
+  FO_CHECK(N >= 8 && N % 8 == 0 && N <= INT32_MAX, "N must be a multiple of 8 (N=", N, ")");
   FO_CHECK(SB.is_cuda() && SB.is_contiguous() && SB.scalar_type() == at::kFloat && SB.dim() == (grouped ? 2 : 1) &&
                SB.numel() == E * N && SB.size(-1) == N,
            grouped ? "SB must be a contiguous float32 CUDA tensor [experts, N]" : "SB must be a contiguous float32 CUDA tensor [N]");
-  FO_CHECK(C.is_cuda() && C.is_contiguous() && (C.scalar_type() == at::kBFloat16 || C.scalar_type() == at::kHalf) &&
-               C.dim() == 2 && C.size(0) == M && C.size(1) == N,
-           "C must be a contiguous bfloat16 or float16 CUDA tensor [M, N]");
   if (grouped) {
     FO_CHECK(E >= 1 && E <= kI8MaxExperts, "1 to ", kI8MaxExperts, " experts (", E, ")");
     FO_CHECK(offsets->is_cuda() && offsets->is_contiguous() && offsets->scalar_type() == at::kInt && offsets->dim() == 1 &&
                  offsets->size(0) == E + 1,
              "offsets must be a contiguous int32 CUDA tensor [experts + 1]");
-    check_device(*offsets, A, "offsets");
-    FO_CHECK(!overlaps(C, C.numel(), *offsets, offsets->numel()), "C must not overlap offsets");
+    check_device(*offsets, like, "offsets");
   }
-  check_device(B, A, "B");
-  check_device(SA, A, "SA");
-  check_device(SB, A, "SB");
-  check_device(C, A, "C");
-  check_aligned(SB.data_ptr(), "SB");
-  check_aligned(A.data_ptr(), "A");
+  check_device(B, like, "B");
+  check_device(SB, like, "SB");
   check_aligned(B.data_ptr(), "B");
+  check_aligned(SB.data_ptr(), "SB");
+  std::memset(p, 0, sizeof(*p));
+  p->N = static_cast<int>(N);
+  p->K = static_cast<int>(K);
+  p->experts = static_cast<int>(E);
+  p->offsets = grouped ? offsets->data_ptr<int>() : nullptr;
+  p->SB = SB.data_ptr<float>();
+}
+
+// C [p->M, p->N] from the 8-bit rows A and their scales SA.
+void OverlapImpl::run_i8(GemmI8Params* p, const void* A, const float* SA, const void* B, void* C, bool bf16, int device) {
+  FO_CHECK(world_ == 1, "8-bit products are single-rank calls");
+  if (heap_ == nullptr) NcclInit(0, 1, {});
+  FO_CHECK(device == device_, "the operands are on another device than this object");
+  p->SA = SA;
+  p->C = static_cast<uint16_t*>(C);
+  p->status = status_.data_ptr<int>();
+  p->timeout_ns = static_cast<uint64_t>(opt_timeout_ms_) * 1000000ull;
+  const GemmI8Plan plan = choose_i8(p->M, p->N, p->K, p->experts, p->offsets != nullptr);
+  const std::string e = gemm_i8_launch(plan, *p, A, B, bf16, stream());
+  FO_CHECK(e.empty(), "gemm_i8: ", e, " (M=", p->M, " N=", p->N, " K=", p->K, " experts=", p->experts, ")");
+}
+
+void OverlapImpl::GemmI8(at::Tensor A, at::Tensor B, at::Tensor SA, at::Tensor SB, at::Tensor C,
+                         c10::optional<at::Tensor> offsets) {
+  NvtxRange nvtx_range("flashoverlap::gemm_i8");
+  FO_CHECK(A.is_cuda() && A.dim() == 2 && A.is_contiguous() && A.scalar_type() == at::kChar,
+           "A must be a contiguous int8 CUDA tensor [M, K]");
+  GemmI8Params p;
+  check_i8_weights(A, A.size(1), B, SB, offsets, &p);
+  const int64_t M = A.size(0);
+  FO_CHECK(M <= INT32_MAX, "too many rows");
+  FO_CHECK(SA.is_cuda() && SA.is_contiguous() && SA.scalar_type() == at::kFloat && SA.dim() == 1 && SA.size(0) == M,
+           "SA must be a contiguous float32 CUDA tensor [M]");
+  FO_CHECK(C.is_cuda() && C.is_contiguous() && (C.scalar_type() == at::kBFloat16 || C.scalar_type() == at::kHalf) &&
+               C.dim() == 2 && C.size(0) == M && C.size(1) == p.N,
+           "C must be a contiguous bfloat16 or float16 CUDA tensor [M, N]");
+  check_device(SA, A, "SA");
+  check_device(C, A, "C");
+  check_aligned(A.data_ptr(), "A");
   check_aligned(C.data_ptr(), "C");
   FO_CHECK(!overlaps(C, C.numel(), A, A.numel()) && !overlaps(C, C.numel(), B, B.numel()) &&
-               !overlaps(C, C.numel(), SA, SA.numel()) && !overlaps(C, C.numel(), SB, SB.numel()),
-           "C must not overlap A, B, SA or SB");
+               !overlaps(C, C.numel(), SA, SA.numel()) && !overlaps(C, C.numel(), SB, SB.numel()) &&
+               (p.offsets == nullptr || !overlaps(C, C.numel(), *offsets, offsets->numel())),
+           "C must not overlap A, B, SA, SB or offsets");
   if (M == 0) return;
   c10::cuda::CUDAGuard guard(A.device());
-  if (heap_ == nullptr) NcclInit(0, 1, {});
-  FO_CHECK(A.get_device() == device_, "the operands are on another device than this object");
-  GemmI8Params p;
-  std::memset(&p, 0, sizeof(p));
   p.M = static_cast<int>(M);
-  p.N = static_cast<int>(N);
-  p.K = static_cast<int>(K);
-  p.experts = static_cast<int>(E);
-  p.offsets = grouped ? offsets->data_ptr<int>() : nullptr;
-  p.SA = SA.data_ptr<float>();
-  p.SB = SB.data_ptr<float>();
-  p.C = static_cast<uint16_t*>(C.data_ptr());
-  p.status = status_.data_ptr<int>();
-  p.timeout_ns = static_cast<uint64_t>(opt_timeout_ms_) * 1000000ull;
-  const GemmI8Plan plan = choose_i8(p.M, p.N, p.K, p.experts, grouped);
-  const std::string e = gemm_i8_launch(plan, p, A.data_ptr(), B.data_ptr(), C.scalar_type() == at::kBFloat16, stream());
-  FO_CHECK(e.empty(), "gemm_i8: ", e, " (M=", M, " N=", N, " K=", K, " experts=", E, ")");
+  run_i8(&p, A.data_ptr(), SA.data_ptr<float>(), B.data_ptr(), C.data_ptr(), C.scalar_type() == at::kBFloat16, A.get_device());
 }
 
 at::Tensor OverlapImpl::LinearI8(at::Tensor X, at::Tensor B, at::Tensor SB, c10::optional<at::Tensor> offsets) {
   NvtxRange nvtx_range("flashoverlap::linear_i8");
   FO_CHECK(X.is_cuda() && (X.scalar_type() == at::kBFloat16 || X.scalar_type() == at::kHalf) && X.dim() >= 1,
            "X must be a bfloat16 or float16 CUDA tensor [..., K]");
-  FO_CHECK(B.dim() >= 2 && X.size(-1) == B.size(-1), "X [..., K] and B disagree on K");
-  const int64_t K = X.size(-1), N = B.size(-2);
-  FO_CHECK(K >= 16 && K % 16 == 0 && K <= kMaxQuantizeDim, "K must be a multiple of 16 from 16 to ", kMaxQuantizeDim, " (K=", K, ")");
+  GemmI8Params p;
+  check_i8_weights(X, X.size(-1), B, SB, offsets, &p);
+  const int64_t K = p.K;
+  FO_CHECK(K <= kMaxQuantizeDim, "K must be a multiple of 16 from 16 to ", kMaxQuantizeDim, " (K=", K, ")");
   c10::cuda::CUDAGuard guard(X.device());
-  at::Tensor x = X.reshape({-1, K}).contiguous();
+  at::Tensor x = X.dim() == 2 && X.is_contiguous() ? X : X.reshape({-1, K}).contiguous();
   if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone();
   const int64_t M = x.size(0);
   FO_CHECK(M <= INT32_MAX, "too many rows");
-  at::Tensor q = at::empty({M, K}, x.options().dtype(at::kChar)), sa = at::empty({M}, x.options().dtype(at::kFloat));
-  at::Tensor c = at::empty({M, N}, x.options());
-  cuda_check(quantize_rows_launch(x.data_ptr(), q.data_ptr(), sa.data_ptr<float>(), static_cast<int>(M), static_cast<int>(K),
-                                  x.scalar_type() == at::kBFloat16, stream()),
-             "quantize_rows");
-  GemmI8(q, B, sa, SB, c, offsets);
+  p.M = static_cast<int>(M);
+  const bool bf16 = x.scalar_type() == at::kBFloat16;
+  at::Tensor c = at::empty({M, p.N}, x.options());
+  if (M > 0) {
+    // the 8-bit rows and behind them their scales (K is a multiple of 16, so those are aligned)
+    at::Tensor rows = at::empty({M * (K + 4)}, x.options().dtype(at::kChar));
+    float* scales = reinterpret_cast<float*>(static_cast<char*>(rows.data_ptr()) + M * K);
+    cuda_check(quantize_rows_launch(x.data_ptr(), rows.data_ptr(), scales, p.M, p.K, bf16, stream()), "quantize_rows");
+    run_i8(&p, rows.data_ptr(), scales, B.data_ptr(), c.data_ptr(), bf16, x.get_device());
+  }
   if (X.dim() == 2) return c;
   std::vector<int64_t> sizes = X.sizes().vec();
-  sizes.back() = N;
+  sizes.back() = p.N;
   return c.view(sizes);
 }
 

@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "../comm/symmetric_heap.h"
+#include "../gemm/fo_gemm_i8.h"
 #include "../gemm/fo_gemm_params.h"
 
 namespace fo {
@@ -169,6 +170,7 @@ class OverlapImpl : public torch::CustomClassHolder {
                           bool monitor, bool needs_counters) const;
   void ensure_comm_stream();
   cudaStream_t stream() const;
+  void run_i8(GemmI8Params* p, const void* A, const float* SA, const void* B, void* C, bool bf16, int device);
   ncclDataType_t nccl_dtype(const at::Tensor& t) const;
 
   int rank_ = 0;
