@@ -2,6 +2,7 @@
 // torch.ops.flashoverlap_op.*, with the reference's method names and argument orders
 // (src/pybind.cpp:114-150) plus the additions this library makes (marked below).
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -140,9 +141,29 @@ c10::optional<at::Tensor> or_none(const at::Tensor& t) { return t.defined() ? c1
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// A leaf's gradient is accumulated on the stream of the first live graph that it is part of.  A backward pass that is being
+// captured would pull that stream into the capture, which ends the process inside the engine: refused here, in the forward pass.
+void check_leaf_in_capture(const at::Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (accumulator == nullptr) return;
+  const auto stream = accumulator->stream();
+  FO_CHECK(!stream.has_value() || *stream == c10::cuda::getCurrentCUDAStream(t.get_device()).unwrap(),
+           "a tensor that requires a gradient is part of a live graph of another stream than the one being captured: ",
+           "release that graph (its loss and outputs) before the capture");
+}
+
+// Whether a call has a gradient to record.
 template <typename... T>
 bool records(const T&... t) {
-  return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
+  if (!at::GradMode::is_enabled() || !((t.defined() && t.requires_grad()) || ...)) return false;
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) (check_leaf_in_capture(t), ...);
+  return true;
+}
+
+template <typename... T>
+void check_no_gradient(const char* what, const T&... t) {
+  FO_CHECK(!at::GradMode::is_enabled() || !(t.requires_grad() || ...), what, " has no gradient: call it under no_grad, or detach its inputs");
 }
 
 // Gradients whose own derivatives do not exist: with a graph being recorded for them, differentiating it raises.
@@ -442,6 +463,7 @@ at::Tensor moe_combine(at::Tensor R, c10::optional<at::Tensor> weights, at::Tens
 
 // (Q int8, S fp32 [rows]) of X [rows, dim].
 std::tuple<at::Tensor, at::Tensor> quantize_rows(at::Tensor X) {
+  check_no_gradient("quantize_rows", X);
   check_16bit(X, "X");
   FO_CHECK(X.dim() == 2 && X.size(0) <= INT32_MAX, "X must be [rows, dim]");
   FO_CHECK(X.size(1) >= 8 && X.size(1) % 8 == 0 && X.size(1) <= fo::kMaxQuantizeDim, "dim must be a multiple of 8 from 8 to ",

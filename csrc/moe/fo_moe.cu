@@ -17,8 +17,9 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-// Choices up to which one CTA sorts, and from which on sixteen do and `source` is written by all SMs; between them eight.
-constexpr int kSortOne = 4096, kSortMany = 32768;
+// Choices up to which one CTA sorts, and eight; sixteen from there on.
+constexpr int kSortOne = 512, kSortEight = 8192;
+constexpr int kSortBatch = 4;
 
 __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {
   uint32_t v;
@@ -30,8 +31,7 @@ __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr)
 // expert in a row of its own in shared memory; the counts of the warps and, through distributed shared memory, of the CTAs in
 // front of it give each warp its first row for every expert, and a second walk over the same run hands the rows out, 32
 // choices a step: ballots over the expert's bits tell each lane which others have its expert (half the time of match.any, whose
-// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us).  Bound by latency, and for many
-// choices by the scattered stores of `source`, which then all SMs do in a launch of their own.
+// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us with eight CTAs).  Bound by latency.
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     moe_sort_kernel(const Id* __restrict__ ids, int64_t n, int experts, int32_t* __restrict__ slot,
@@ -57,11 +57,15 @@ __global__ void __launch_bounds__(kSortThreads)
     const Id v = ids[i];
     return v >= 0 && v < static_cast<Id>(experts) ? static_cast<int>(v) : experts;
   };
-  int next = expert_at(begin + lane);
-  for (int64_t i = begin; i < end; i += 32) {
-    const int e = next;
-    next = expert_at(i + 32 + lane);
-    if (e < experts) atomicAdd(mine + e, 1u);  // a count does not depend on the order
+  // the walks go in batches whose loads are in flight together
+  for (int64_t i0 = begin; i0 < end; i0 += 32 * kSortBatch) {
+    int ex[kSortBatch];
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) ex[u] = expert_at(i0 + 32 * u + lane);
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) {
+      if (ex[u] < experts) atomicAdd(mine + ex[u], 1u);  // a count does not depend on the order
+    }
   }
   __syncthreads();
   const int e = threadIdx.x;  // experts <= kSortThreads
@@ -115,45 +119,36 @@ __global__ void __launch_bounds__(kSortThreads)
   if (rank == 0 && threadIdx.x == 0) offsets[experts] = static_cast<int32_t>(rows);
   __syncthreads();
   const int bits = 32 - __clz(experts);
-  next = expert_at(begin + lane);
-  for (int64_t i = begin; i < end; i += 32) {
-    const int ex = next;
-    next = expert_at(i + 32 + lane);
-    uint32_t same = 0xffffffffu;  // the lanes with this lane's expert
-    for (int b = 0; b < bits; ++b) {
-      const uint32_t ones = __ballot_sync(0xffffffffu, (ex >> b) & 1);
-      same &= (ex >> b) & 1 ? ones : ~ones;
+  for (int64_t i0 = begin; i0 < end; i0 += 32 * kSortBatch) {
+    int batch[kSortBatch];
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) batch[u] = expert_at(i0 + 32 * u + lane);
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) {
+      if (i0 + 32 * u >= end) break;
+      const int ex = batch[u];
+      uint32_t same = 0xffffffffu;  // the lanes with this lane's expert
+      for (int b = 0; b < bits; ++b) {
+        const uint32_t ones = __ballot_sync(0xffffffffu, (ex >> b) & 1);
+        same &= (ex >> b) & 1 ? ones : ~ones;
+      }
+      const int64_t i = i0 + 32 * u + lane;
+      int32_t row = -1;
+      if (ex < experts) {
+        row = static_cast<int32_t>(mine[ex] + __popc(same & ((1u << lane) - 1u)));
+        source[row] = static_cast<int32_t>(i);
+      }
+      __syncwarp();
+      if (ex < experts && lane == __ffs(same) - 1) mine[ex] += __popc(same);
+      __syncwarp();
+      if (i < end) slot[i] = row;
     }
-    int32_t row = -1;
-    if (ex < experts) {
-      row = static_cast<int32_t>(mine[ex] + __popc(same & ((1u << lane) - 1u)));
-      if (source != nullptr) source[row] = static_cast<int32_t>(i + lane);
-    }
-    __syncwarp();
-    if (ex < experts && lane == __ffs(same) - 1) mine[ex] += __popc(same);
-    __syncwarp();
-    if (i + lane < end) slot[i + lane] = row;
   }
-  if (source != nullptr) {
-    for (int64_t r = rows + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n; r += static_cast<int64_t>(ctas) * kSortThreads) {
-      source[r] = -1;
-    }
+  for (int64_t r = rows + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n; r += static_cast<int64_t>(ctas) * kSortThreads) {
+    source[r] = -1;
   }
   __syncwarp();
   ptx::cluster_wait_acquire();
-}
-
-// source[slot[i]] = i, and -1 behind the last row.
-__global__ void __launch_bounds__(256)
-    moe_source_kernel(const int32_t* __restrict__ slot, const int32_t* __restrict__ offsets, int32_t* __restrict__ source,
-                      int n, int experts) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  ptx::grid_launch_dependents();
-  ptx::grid_wait();
-  if (i >= n) return;
-  const int row = slot[i];
-  if (row >= 0) source[row] = static_cast<int32_t>(i);
-  if (i >= offsets[experts]) source[i] = -1;
 }
 
 // ---------------------------------------------------------------------------- the rows
@@ -406,8 +401,7 @@ cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, 
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 16) set[dev] = true;
   }
-  const bool many = n > kSortMany;
-  const int ctas = n <= kSortOne ? 1 : (many ? 16 : 8);
+  const int ctas = n <= kSortOne ? 1 : (n <= kSortEight ? 8 : 16);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -422,11 +416,9 @@ cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), n, experts, slot, many ? nullptr : source, offsets);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), n, experts, slot, source, offsets);
   if (e != cudaSuccess) cudaGetLastError();
-  if (e != cudaSuccess || !many) return e;
-  return launch(moe_source_kernel, (n + 255) / 256, 256, stream, static_cast<const int32_t*>(slot), static_cast<const int32_t*>(offsets),
-                source, static_cast<int>(n), experts);
+  return e;
 }
 
 bool valid(const MoeShape& s) {

@@ -476,7 +476,13 @@ static void check_i8_weights(const at::Tensor& like, int64_t K, const at::Tensor
 // C [p->M, p->N] from the 8-bit rows A and their scales SA.
 void OverlapImpl::run_i8(GemmI8Params* p, const void* A, const float* SA, const void* B, void* C, bool bf16, int device) {
   FO_CHECK(world_ == 1, "8-bit products are single-rank calls");
-  if (heap_ == nullptr) NcclInit(0, 1, {});
+  if (heap_ == nullptr) {
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    cuda_check(cudaStreamIsCapturing(stream(), &capturing), "cudaStreamIsCapturing");
+    FO_CHECK(capturing == cudaStreamCaptureStatusNone, "call nccl_init or cutlass_init before a capture: ",
+             "the object's status words would be the graph's");
+    NcclInit(0, 1, {});
+  }
   FO_CHECK(device == device_, "the operands are on another device than this object");
   p->SA = SA;
   p->C = static_cast<uint16_t*>(C);
@@ -517,6 +523,8 @@ void OverlapImpl::GemmI8(at::Tensor A, at::Tensor B, at::Tensor SA, at::Tensor S
 
 at::Tensor OverlapImpl::LinearI8(at::Tensor X, at::Tensor B, at::Tensor SB, c10::optional<at::Tensor> offsets) {
   NvtxRange nvtx_range("flashoverlap::linear_i8");
+  FO_CHECK(!at::GradMode::is_enabled() || !(X.requires_grad() || SB.requires_grad()),
+           "linear_i8 has no gradient: call it under no_grad, or detach its inputs");
   FO_CHECK(X.is_cuda() && (X.scalar_type() == at::kBFloat16 || X.scalar_type() == at::kHalf) && X.dim() >= 1,
            "X must be a bfloat16 or float16 CUDA tensor [..., K]");
   GemmI8Params p;

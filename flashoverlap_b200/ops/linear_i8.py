@@ -14,8 +14,6 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
     ``dim`` is a multiple of 8 up to 32768.  A row with a NaN or an infinity gets zeros and the scale NaN, so that
     what is computed from it is NaN."""
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("quantize_rows has no gradient: detach its input")
     return native("quantize_rows")(x)
 
 
@@ -28,6 +26,4 @@ def linear_i8(impl, x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     ``offsets`` (``ExpertOrder.offsets``) ``weight`` is [experts, N, K] and ``weight_scale`` [experts, N]: rows
     ``offsets[e]`` to ``offsets[e + 1] - 1`` of ``x`` [rows, K] are multiplied by ``weight[e]``, other rows of the result are zero.
     The sums are exact; nothing here has a gradient."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad):
-        raise RuntimeError("linear_i8 has no gradient: call it under no_grad, or detach its inputs")
     return impl.linear_i8(x, weight, weight_scale, offsets)
