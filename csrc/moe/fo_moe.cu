@@ -37,15 +37,18 @@ __global__ void __launch_bounds__(kSortThreads)
     moe_sort_kernel(const Id* __restrict__ ids, int64_t n, int experts, int32_t* __restrict__ slot,
                     int32_t* __restrict__ source, int32_t* __restrict__ offsets) {
   extern __shared__ uint32_t smem[];
-  uint32_t* count = smem;                       // [kSortWarps][experts], then the next row of each
-  uint32_t* total = count + kSortWarps * experts;  // [experts]: this CTA's choices
+  uint32_t* total = smem;              // [experts]: this CTA's choices
+  uint32_t* base = total + experts;    // [experts]: the first row of these
+  uint32_t* count = base + experts;    // [kSortWarps][experts]: each warp's, then its next row behind the first
   __shared__ uint32_t scan[kSortWarps];
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int ctas = static_cast<int>(gridDim.x);  // one cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* mine = count + warp * experts;
-  for (int e = threadIdx.x; e < kSortWarps * experts; e += kSortThreads) count[e] = 0;
   const int64_t per_warp = (n + ctas * kSortThreads - 1) / (ctas * kSortThreads) * 32;
+  const int64_t left = n - static_cast<int64_t>(rank) * kSortWarps * per_warp;
+  const int warps_used = left <= 0 ? 0 : static_cast<int>(min((left + per_warp - 1) / per_warp, static_cast<int64_t>(kSortWarps)));
+  for (int e = threadIdx.x; e < warps_used * experts; e += kSortThreads) count[e] = 0;
   const int64_t begin = min(n, (static_cast<int64_t>(rank) * kSortWarps + warp) * per_warp);
   const int64_t end = min(n, begin + per_warp);
   ptx::grid_launch_dependents();
@@ -72,18 +75,22 @@ __global__ void __launch_bounds__(kSortThreads)
   if (e < experts) {
     uint32_t sum = 0;
 #pragma unroll 8
-    for (int w = 0; w < kSortWarps; ++w) {
+    for (int w = 0; w < warps_used; ++w) {
       const uint32_t c = count[w * experts + e];
       count[w * experts + e] = sum;
       sum += c;
     }
     total[e] = sum;
   }
-  __syncwarp();  // the barrier's aligned forms take whole warps
-  ptx::cluster_arrive_release();
-  ptx::cluster_wait_acquire();
   uint32_t before = 0, all = 0;
-  if (e < experts) {
+  if (ctas > 1) {
+    __syncwarp();  // the barrier's aligned forms take whole warps
+    ptx::cluster_arrive_release();
+    ptx::cluster_wait_acquire();
+  }
+  if (e < experts && ctas == 1) {
+    all = total[e];
+  } else if (e < experts) {
     for (int c = 0; c < ctas; ++c) {
       const uint32_t v = ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(total + e), c));
       if (c < rank) before += v;
@@ -92,7 +99,7 @@ __global__ void __launch_bounds__(kSortThreads)
   }
   // nobody reads another CTA's counts from here on
   __syncwarp();
-  ptx::cluster_arrive_relaxed();
+  if (ctas > 1) ptx::cluster_arrive_relaxed();
   // exclusive sums over the experts
   uint32_t incl = all;
 #pragma unroll
@@ -113,8 +120,7 @@ __global__ void __launch_bounds__(kSortThreads)
   const uint32_t first = incl - all + (warp > 0 ? in_front : 0u);
   if (e < experts) {
     if (rank == 0) offsets[e] = static_cast<int32_t>(first);
-#pragma unroll 8
-    for (int w = 0; w < kSortWarps; ++w) count[w * experts + e] += first + before;
+    base[e] = first + before;
   }
   if (rank == 0 && threadIdx.x == 0) offsets[experts] = static_cast<int32_t>(rows);
   __syncthreads();
@@ -135,7 +141,7 @@ __global__ void __launch_bounds__(kSortThreads)
       const int64_t i = i0 + 32 * u + lane;
       int32_t row = -1;
       if (ex < experts) {
-        row = static_cast<int32_t>(mine[ex] + __popc(same & ((1u << lane) - 1u)));
+        row = static_cast<int32_t>(base[ex] + mine[ex] + __popc(same & ((1u << lane) - 1u)));
         source[row] = static_cast<int32_t>(i);
       }
       __syncwarp();
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(kSortThreads)
     source[r] = -1;
   }
   __syncwarp();
-  ptx::cluster_wait_acquire();
+  if (ctas > 1) ptx::cluster_wait_acquire();
 }
 
 // ---------------------------------------------------------------------------- the rows
@@ -390,13 +396,13 @@ template <typename Id>
 cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, int32_t* source, int32_t* offsets,
                         cudaStream_t stream) {
   auto kernel = moe_sort_kernel<Id>;
-  const int smem = (kSortWarps + 1) * experts * static_cast<int>(sizeof(uint32_t));
+  const int smem = (kSortWarps + 2) * experts * static_cast<int>(sizeof(uint32_t));
   static bool set[16] = {};  // the same whoever sets it
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (kSortWarps + 1) * kMaxExperts * static_cast<int>(sizeof(uint32_t)));
+                                         (kSortWarps + 2) * kMaxExperts * static_cast<int>(sizeof(uint32_t)));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 16) set[dev] = true;

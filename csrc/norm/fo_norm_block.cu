@@ -94,6 +94,8 @@ __device__ __forceinline__ float4 row_sums(const float4& v, float (*red)[128], i
 
 __device__ __forceinline__ uint4 ld_vec(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
+__device__ __forceinline__ void prefetch_l1(const uint16_t* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // The rows a thread reads come through a ring in shared memory that it fills with asynchronous copies, STAGES - 1 rows
 // ahead.  Every thread copies and reads words of its own only, so the ring needs no barrier, and the loads in
 // flight take no registers.
@@ -186,6 +188,18 @@ __global__ void __launch_bounds__(kMaxThreads, 2)
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s) fill(s, row_begin + s);
+  // what the first row wants next of the weights, so that one row by itself waits for memory once
+  if ((threadIdx.x & 7) == 0) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int at_vec = c.first + i * c.step;
+      if (at_vec < dim) {
+        prefetch_l1(PW + at_vec);
+        prefetch_l1(W + at_vec);
+        if constexpr (GATE == kLineGate) prefetch_l1(G + static_cast<size_t>(row_begin / rows_per_line) * dim + at_vec);
+      }
+    }
+  }
   int stage = 0;
   [[maybe_unused]] int line = row_begin / rows_per_line;
   [[maybe_unused]] int line_left = (line + 1) * rows_per_line - row_begin;  // rows of the gate's line that are left
