@@ -225,9 +225,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_block_forward(at::Tensor X, 
   check_16bit(X, "X");
   c10::cuda::CUDAGuard guard(X.device());
   const NormBlockOperands o = norm_block_operands(X, T, PW, W, G, alpha, eps);
-  at::Tensor H = at::empty(X.sizes(), o.X.options()), Y = at::empty(X.sizes(), o.X.options());
+  const at::ScalarType type = o.X.scalar_type();
+  at::Tensor H = fo::fresh(X.sizes(), type, X), Y = fo::fresh(X.sizes(), type, X);
   at::Tensor stats;
-  if (with_stats) stats = at::empty({X.size(0), 2}, o.X.options().dtype(at::kFloat));
+  if (with_stats) stats = fo::fresh({X.size(0), 2}, at::kFloat, X);
   if (o.p.rows > 0) {
     fo::cuda_check(fo::norm_block_launch(o.p, H.data_ptr(), Y.data_ptr(), with_stats ? stats.data_ptr<float>() : nullptr,
                                          sm_count_of_current_device(), c10::cuda::getCurrentCUDAStream().stream()),
@@ -255,14 +256,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm_a
                stats.size(0) == X.size(0) && stats.size(1) == 2,
            "stats must be what the forward pass returned");
   fo::check_device(stats, X, "stats");
-  const auto options = o.X.options();
-  at::Tensor DX = at::empty(X.sizes(), options), DT = at::empty(X.sizes(), options);
+  const at::ScalarType type = o.X.scalar_type();
+  at::Tensor DX = fo::fresh(X.sizes(), type, X), DT = fo::fresh(X.sizes(), type, X);
   const bool none = o.p.rows == 0;
-  at::Tensor DPW = none ? at::zeros_like(o.PW) : at::empty_like(o.PW), DW = none ? at::zeros_like(o.W) : at::empty_like(o.W);
-  at::Tensor DG = !o.G.defined() ? at::empty({0}, options) : (none ? at::zeros_like(o.G) : at::empty_like(o.G));
+  at::Tensor DPW = none ? at::zeros_like(o.PW) : fo::fresh(PW.sizes(), type, X), DW = none ? at::zeros_like(o.W) : fo::fresh(W.sizes(), type, X);
+  at::Tensor DG = !o.G.defined() ? fo::fresh({0}, type, X) : (none ? at::zeros_like(o.G) : fo::fresh(o.G.sizes(), type, X));
   if (!none) {
     const fo::NormBlockPlan plan = fo::norm_block_plan(o.p, sm_count_of_current_device());
-    at::Tensor workspace = at::empty({static_cast<int64_t>(plan.workspace)}, options.dtype(at::kFloat));
+    at::Tensor workspace = fo::fresh({static_cast<int64_t>(plan.workspace)}, at::kFloat, X);
     fo::cuda_check(fo::norm_block_backward_launch(o.p, stats.data_ptr<float>(), gh.defined() ? gh.data_ptr() : nullptr,
                                                   gy.defined() ? gy.data_ptr() : nullptr, DX.data_ptr(), DT.data_ptr(),
                                                   DPW.data_ptr(), DW.data_ptr(), DG.data_ptr(), workspace.data_ptr<float>(),
@@ -315,9 +316,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_sort(at::Tensor ids, int64_t 
   FO_CHECK(ids.numel() <= INT32_MAX, "too many choices");
   c10::cuda::CUDAGuard guard(ids.device());
   const at::Tensor c = ids.contiguous();
-  const auto options = c.options().dtype(at::kInt);
-  at::Tensor slot = at::empty(ids.sizes(), options), source = at::empty({ids.numel()}, options);
-  at::Tensor offsets = at::empty({experts + 1}, options);
+  at::Tensor slot = fo::fresh(ids.sizes(), at::kInt, ids), source = fo::fresh({ids.numel()}, at::kInt, ids);
+  at::Tensor offsets = fo::fresh({experts + 1}, at::kInt, ids);
   fo::cuda_check(fo::moe_sort_launch(c.data_ptr(), c.scalar_type() == at::kLong, c.numel(), static_cast<int>(experts),
                                      slot.data_ptr<int>(), source.data_ptr<int>(), offsets.data_ptr<int>(),
                                      c10::cuda::getCurrentCUDAStream().stream()),
@@ -364,7 +364,7 @@ at::Tensor dispatch_rows(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
   c10::cuda::CUDAGuard guard(X.device());
   const fo::MoeShape s = moe_shape(X, X.size(1), slot, &offsets);
   const at::Tensor x = dense(X);
-  at::Tensor R = at::empty({slot.numel(), X.size(1)}, x.options());
+  at::Tensor R = fo::fresh({slot.numel(), X.size(1)}, X.scalar_type(), X);
   if (s.tokens > 0) {
     fo::cuda_check(fo::moe_dispatch_launch(s, x.data_ptr(), slot.data_ptr<int>(), offsets.data_ptr<int>(), R.data_ptr(),
                                            c10::cuda::getCurrentCUDAStream().stream()),
@@ -380,7 +380,7 @@ at::Tensor combine_rows(at::Tensor R, c10::optional<at::Tensor> weights, at::Ten
   c10::cuda::CUDAGuard guard(R.device());
   const fo::MoeShape s = moe_shape(R, R.size(1), slot, offsets);
   const at::Tensor r = dense(R), w = moe_weights(weights, R, slot);
-  at::Tensor O = at::empty({slot.size(0), R.size(1)}, r.options());
+  at::Tensor O = fo::fresh({slot.size(0), R.size(1)}, R.scalar_type(), R);
   if (s.tokens > 0) {
     fo::cuda_check(fo::moe_combine_launch(s, r.data_ptr(), weights_arg(w), slot.data_ptr<int>(), O.data_ptr(),
                                           c10::cuda::getCurrentCUDAStream().stream()),
@@ -407,8 +407,8 @@ std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::opti
     fo::check_device(*R, GO, "R");
     r = dense(*R);
   }
-  DR = at::empty({for_rows ? slot.numel() : 0, GO.size(1)}, go.options());
-  DW = for_weights ? at::empty(slot.sizes(), w.options()) : at::empty({0}, go.options());
+  DR = fo::fresh({for_rows ? slot.numel() : 0, GO.size(1)}, GO.scalar_type(), GO);
+  DW = for_weights ? fo::fresh(slot.sizes(), w.scalar_type(), GO) : fo::fresh({0}, GO.scalar_type(), GO);
   if (s.tokens > 0) {
     fo::cuda_check(fo::moe_combine_backward_launch(s, go.data_ptr(), r.defined() ? r.data_ptr() : nullptr, weights_arg(w),
                                                    slot.data_ptr<int>(), offsets.data_ptr<int>(),
@@ -470,7 +470,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(at::Tensor X) {
            fo::kMaxQuantizeDim, " (", X.size(1), ")");
   c10::cuda::CUDAGuard guard(X.device());
   const at::Tensor x = dense(X);
-  at::Tensor Q = at::empty(X.sizes(), x.options().dtype(at::kChar)), S = at::empty({X.size(0)}, x.options().dtype(at::kFloat));
+  at::Tensor Q = fo::fresh(X.sizes(), at::kChar, X), S = fo::fresh({X.size(0)}, at::kFloat, X);
   fo::cuda_check(fo::quantize_rows_launch(x.data_ptr(), Q.data_ptr(), S.data_ptr<float>(), static_cast<int>(X.size(0)),
                                           static_cast<int>(X.size(1)), x.scalar_type() == at::kBFloat16,
                                           c10::cuda::getCurrentCUDAStream().stream()),

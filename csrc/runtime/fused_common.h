@@ -2,6 +2,7 @@
 // symmetric "signal" region, operand checks and the GemmParams set-up of one call.
 #pragma once
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 
@@ -69,6 +70,11 @@ inline bool overlaps(const at::Tensor& a, int64_t a_numel, const at::Tensor& b, 
   const auto a0 = reinterpret_cast<uintptr_t>(a.data_ptr()), b0 = reinterpret_cast<uintptr_t>(b.data_ptr());
   return a0 < b0 + static_cast<uintptr_t>(b_numel) * b.element_size() &&
          b0 < a0 + static_cast<uintptr_t>(a_numel) * a.element_size();
+}
+
+// A new tensor on `like`'s device, straight from the allocator.
+inline at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
 }
 
 inline const int* int_ptr_or_null(const at::Tensor& t, const char* name) {

@@ -538,10 +538,10 @@ at::Tensor OverlapImpl::LinearI8(at::Tensor X, at::Tensor B, at::Tensor SB, c10:
   FO_CHECK(M <= INT32_MAX, "too many rows");
   p.M = static_cast<int>(M);
   const bool bf16 = x.scalar_type() == at::kBFloat16;
-  at::Tensor c = at::empty({M, p.N}, x.options());
+  at::Tensor c = fresh({M, p.N}, x.scalar_type(), x);
   if (M > 0) {
     // the 8-bit rows and behind them their scales (K is a multiple of 16, so those are aligned)
-    at::Tensor rows = at::empty({M * (K + 4)}, x.options().dtype(at::kChar));
+    at::Tensor rows = fresh({M * (K + 4)}, at::kChar, x);
     float* scales = reinterpret_cast<float*>(static_cast<char*>(rows.data_ptr()) + M * K);
     cuda_check(quantize_rows_launch(x.data_ptr(), rows.data_ptr(), scales, p.M, p.K, bf16, stream()), "quantize_rows");
     run_i8(&p, rows.data_ptr(), scales, B.data_ptr(), c.data_ptr(), bf16, x.get_device());
