@@ -94,8 +94,6 @@ __device__ __forceinline__ float4 row_sums(const float4& v, float (*red)[128], i
 
 __device__ __forceinline__ uint4 ld_vec(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
-__device__ __forceinline__ void prefetch_l1(const uint16_t* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
-
 // The rows a thread reads come through a ring in shared memory that it fills with asynchronous copies, STAGES - 1 rows
 // ahead.  Every thread copies and reads words of its own only, so the ring needs no barrier, and the loads in
 // flight take no registers.
@@ -127,7 +125,7 @@ enum Gate { kNoGate, kLineGate, kRowGate };
 constexpr int kMinLineRows = 8;
 
 template <int VPT, int GATE>
-using ForwardRing = RowRing<VPT, GATE == kRowGate ? 3 : 2, 2>;
+using ForwardRing = RowRing<VPT, GATE == kRowGate ? 3 : 2, 3>;
 // three stages, two where the gate takes the third's place
 template <int VPT, int GATE>
 using BackwardRing = RowRing<VPT, GATE == kRowGate ? 5 : 4, GATE == kRowGate ? 2 : 3>;
@@ -151,9 +149,12 @@ __device__ __forceinline__ int owner_of_row(int row, int of, int rows) {
   return static_cast<int>(((static_cast<int64_t>(row) + 1) * of - 1) / rows);
 }
 
-// Bound by memory: 8 bytes an element.  A CTA takes a run of rows; a thread owns VPT vectors of a row.
+// Bound by memory: 8 bytes an element.  A CTA takes a run of rows; a thread owns VPT vectors of a row, and what it needs of the
+// weights and of the gate's line stays in its registers: beside the ring there is little L1, and rows that fetched them again
+// from the L2 waited for them (8192 x 4096: 57 -> 47 us, 16384 x 1024: 33 -> 27 us, cold; 16384 x 8192: 183 us either way,
+// 5.9 TB/s).  Rows of one vector a thread leave registers for two sets of CTAs.
 template <bool BF16, int VPT, int CTAS, int GATE>
-__global__ void __launch_bounds__(kMaxThreads, 2)
+__global__ void __launch_bounds__(kMaxThreads, 1)
     norm_block_kernel(const uint16_t* __restrict__ X, const uint16_t* __restrict__ T, const uint16_t* __restrict__ PW,
                       const uint16_t* __restrict__ W, const uint16_t* __restrict__ G, uint16_t* __restrict__ H,
                       uint16_t* __restrict__ Y, float2* __restrict__ stats, int rows, int dim, int rows_per_line,
@@ -188,21 +189,32 @@ __global__ void __launch_bounds__(kMaxThreads, 2)
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s) fill(s, row_begin + s);
-  // what the first row wants next of the weights, so that one row by itself waits for memory once
-  if ((threadIdx.x & 7) == 0) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int at_vec = c.first + i * c.step;
-      if (at_vec < dim) {
-        prefetch_l1(PW + at_vec);
-        prefetch_l1(W + at_vec);
-        if constexpr (GATE == kLineGate) prefetch_l1(G + static_cast<size_t>(row_begin / rows_per_line) * dim + at_vec);
-      }
-    }
-  }
   int stage = 0;
   [[maybe_unused]] int line = row_begin / rows_per_line;
   [[maybe_unused]] int line_left = (line + 1) * rows_per_line - row_begin;  // rows of the gate's line that are left
+  Vec8 pg[VPT];
+  uint4 w16[VPT], pw16[VPT];
+  auto load_line = [&]() {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (c.first + i * c.step < dim) {
+        pg[i] = unpack8<BF16>(ld_vec(PW + c.first + i * c.step));
+        if constexpr (GATE == kLineGate) {
+          const Vec8 g = unpack8<BF16>(ld_vec(G + static_cast<size_t>(line) * dim + c.first + i * c.step));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) pg[i].v[k] = pg[i].v[k] * g.v[k];
+        }
+      }
+    }
+  };
+  if constexpr (GATE != kRowGate) load_line();
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (c.first + i * c.step < dim) {
+      w16[i] = ld_vec(W + c.first + i * c.step);
+      if constexpr (GATE == kRowGate) pw16[i] = ld_vec(PW + c.first + i * c.step);
+    }
+  }
   for (int b = row_begin; b < row_end; ++b) {
     const size_t row = static_cast<size_t>(b) * dim + c.first;
     ring.wait();
@@ -214,12 +226,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2)
     for (int i = 0; i < VPT; ++i) {
       if (c.first + i * c.step < dim) {
         const Vec8 t = unpack8<BF16>(ring.get(stage, 0, i)), x = unpack8<BF16>(ring.get(stage, 1, i));
-        h[i] = unpack8<BF16>(ld_vec(PW + c.first + i * c.step));
-        if constexpr (GATE != kNoGate) {
-          const Vec8 g = unpack8<BF16>(GATE == kRowGate ? ring.get(stage, 2, i)
-                                                        : ld_vec(G + static_cast<size_t>(line) * dim + c.first + i * c.step));
+        if constexpr (GATE == kRowGate) {
+          const Vec8 g = unpack8<BF16>(ring.get(stage, 2, i));
+          h[i] = unpack8<BF16>(pw16[i]);
 #pragma unroll
           for (int k = 0; k < 4; ++k) h[i].v[k] = h[i].v[k] * g.v[k];
+        } else {
+          h[i] = pg[i];
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -261,6 +274,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2)
       if (--line_left == 0) {
         ++line;
         line_left = rows_per_line;
+        if (b + 1 < row_end) load_line();
       }
     }
     const float2 r2 = f2(rsqrtf(hh * inv_dim + eps));
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2)
     for (int i = 0; i < VPT; ++i) {
       if (c.first + i * c.step < dim) {
         __stcs(reinterpret_cast<uint4*>(H + row + i * c.step), pack8<BF16>(h[i]));
-        const Vec8 w = unpack8<BF16>(ld_vec(W + c.first + i * c.step));
+        const Vec8 w = unpack8<BF16>(w16[i]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) h[i].v[k] = h[i].v[k] * r2 * w.v[k];
         __stcs(reinterpret_cast<uint4*>(Y + row + i * c.step), pack8<BF16>(h[i]));
@@ -351,8 +365,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_block_backward_kernel(con
   int stage = 0;
   [[maybe_unused]] int line = row_begin / rows_per_line;
   [[maybe_unused]] int line_end = min(row_end, (line + 1) * rows_per_line);  // of the rows that are this CTA's
-  // What a thread needs of the weights and of the gate's line stays in registers: there is no room for them in the L1 beside
-  // the ring, and a row that fetched them from the L2 waited for them twice.
   const uint16_t* g_line = GATE == kLineGate ? p.G + static_cast<size_t>(line) * dim + c.first : nullptr;
   Vec8 pg[VPT];
   uint4 w16[VPT];
@@ -640,7 +652,7 @@ cudaError_t launch_forward(const NormBlock& p, void* H, void* Y, float* stats, i
   const cudaError_t e = allow_smem(kernel, set);
   if (e != cudaSuccess) return e;
   const int threads = threads_for(p.dim / 8, VPT);
-  const int grid = std::min(p.rows, sm_count / CTAS * std::min(32, 2 * kMaxThreads / threads)) * CTAS;
+  const int grid = std::min(p.rows, sm_count / CTAS * std::min(16, kMaxThreads / threads * (VPT == 1 ? 2 : 1))) * CTAS;
   return launch(kernel, dim3(grid), CTAS, threads, threads * ForwardRing<VPT, GATE>::kBytesPerThread, stream,
                 static_cast<const uint16_t*>(p.X), static_cast<const uint16_t*>(p.T), static_cast<const uint16_t*>(p.PW),
                 static_cast<const uint16_t*>(p.W), static_cast<const uint16_t*>(p.G), static_cast<uint16_t*>(H),
