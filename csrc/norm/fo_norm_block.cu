@@ -189,6 +189,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1)
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s) fill(s, row_begin + s);
+  if constexpr (CTAS > 1) {  // the other CTA runs before anything is stored into its shared memory
+    ptx::cluster_arrive_relaxed();
+    ptx::cluster_wait_acquire();
+  }
   int stage = 0;
   [[maybe_unused]] int line = row_begin / rows_per_line;
   [[maybe_unused]] int line_left = (line + 1) * rows_per_line - row_begin;  // rows of the gate's line that are left
@@ -220,20 +224,24 @@ __global__ void __launch_bounds__(kMaxThreads, 1)
     ring.wait();
     // With q = T PW G, H = alpha X + r1 q, and its sum of squares follows from three sums that do not wait for r1: one
     // exchange between the warps a row instead of two.
+    auto post_gate = [&](int i) {  // PW G
+      if constexpr (GATE == kRowGate) {
+        Vec8 v = unpack8<BF16>(pw16[i]);
+        const Vec8 g = unpack8<BF16>(ring.get(stage, 2, i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v.v[k] = v.v[k] * g.v[k];
+        return v;
+      } else {
+        return pg[i];
+      }
+    };
     Vec8 h[VPT];  // q, then H
     float2 tt = f2(0.f), xx = f2(0.f), xq = f2(0.f), qq = f2(0.f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (c.first + i * c.step < dim) {
         const Vec8 t = unpack8<BF16>(ring.get(stage, 0, i)), x = unpack8<BF16>(ring.get(stage, 1, i));
-        if constexpr (GATE == kRowGate) {
-          const Vec8 g = unpack8<BF16>(ring.get(stage, 2, i));
-          h[i] = unpack8<BF16>(pw16[i]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) h[i].v[k] = h[i].v[k] * g.v[k];
-        } else {
-          h[i] = pg[i];
-        }
+        h[i] = post_gate(i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           h[i].v[k] = h[i].v[k] * t.v[k];
@@ -256,20 +264,26 @@ __global__ void __launch_bounds__(kMaxThreads, 1)
         for (int k = 0; k < 4; ++k) h[i].v[k] = fma2(f2(alpha), x.v[k], h[i].v[k] * f2(r1));
       }
     }
-    fill(stage, b + kStages);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    if (!(hh >= 0.25f * apart)) {
-      // the two parts cancel (or there is no number): a sum of its own, as exact as the parts are
+    if (!(hh >= 0.25f * apart && apart < __int_as_float(0x7f800000))) {
+      // the two parts cancel, or q, which r1 has not scaled yet, is too large to be squared: H in the order of its definition,
+      // and a sum of its own
       float2 ss = f2(0.f);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         if (c.first + i * c.step < dim) {
+          const Vec8 t = unpack8<BF16>(ring.get(stage, 0, i)), x = unpack8<BF16>(ring.get(stage, 1, i));
+          h[i] = post_gate(i);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ss = fma2(h[i].v[k], h[i].v[k], ss);
+          for (int k = 0; k < 4; ++k) {
+            h[i].v[k] = fma2(f2(alpha), x.v[k], t.v[k] * f2(r1) * h[i].v[k]);
+            ss = fma2(h[i].v[k], h[i].v[k], ss);
+          }
         }
       }
       hh = row_sums<CTAS>(make_float4(ss.x + ss.y, 0.f, 0.f, 0.f), red, turn).x;
     }
+    fill(stage, b + kStages);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
     if constexpr (GATE == kLineGate) {
       if (--line_left == 0) {
         ++line;
@@ -361,6 +375,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_block_backward_kernel(con
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s) fill(s, row_begin + s);
+  if constexpr (CTAS > 1) {  // the other CTA runs before anything is stored into its shared memory
+    ptx::cluster_arrive_relaxed();
+    ptx::cluster_wait_acquire();
+  }
   const uint4 zero = make_uint4(0, 0, 0, 0);
   int stage = 0;
   [[maybe_unused]] int line = row_begin / rows_per_line;

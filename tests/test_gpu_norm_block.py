@@ -156,6 +156,41 @@ def test_rows_of_zeros_and_of_what_is_no_number(cuda, dt):
         check(name, got, ref[name], dt, 3)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,dim", [(1, 64), (40, 1032), (20, 8192), (5, 9000)])
+def test_rows_whose_parts_cancel(cuda, dt, rows, dim):
+    """The residual stream undoes the block's output up to what is left of roundings, in every second row."""
+    x, t, pw, w, gv, gh, gy = problem(cuda, dt, rows, dim, "channel")
+    u = reference(torch.zeros_like(x), t, pw, w, gv, 1.0)["h"][0]
+    x[::2] = (-u / 0.7).to(dt)[::2]
+    leaves = [v.requires_grad_() for v in (x, t, pw, w, gv)]
+    h, y = ops.rmsnorm_add_rmsnorm(*leaves, 0.7, EPS)
+    detached = [v.detach() for v in leaves]
+    ref = reference(*detached, 0.7, gh, gy)
+    check("h", h, ref["h"], dt, rows)
+    # 2^-16 of the parts are off in H, and so in its mean square: up to that over H's root mean square, relative, in Y
+    value, (_, hm) = ref["y"][0], ref["h"]
+    rms = ref["h"][0].square().mean(1, keepdim=True).add(EPS).sqrt()
+    off = 2.0 ** -16 * (hm / rms * w.double().abs() + value.abs() * (hm.square().mean(1, keepdim=True).sqrt() / rms))
+    assert ((y.double() - value).abs() <= half_step(dt) * value.abs() + off + smallest(dt)).all()
+    for g in torch.autograd.grad((h, y), leaves, (gh, gy)):
+        assert g.isfinite().all()
+
+
+def test_values_that_only_their_norm_brings_into_range(cuda):
+    """Squares of T fit 32 bits, squares of T with the weights do not."""
+    dt = torch.bfloat16
+    x, t, pw, w, gv, gh, gy = problem(cuda, dt, 12, 2048, "channel")
+    t, gv = t * 1e16, gv * 3e3
+    t[3], t[4] = t[3] * 1e20, 0                     # beyond 32 bits when squared: no part of the block is left, as in 32 bits throughout
+    ref = reference(x, t, pw, w, gv, 1.0)
+    h, y = ops.rmsnorm_add_rmsnorm(x, t, pw, w, gv, 1.0, EPS)
+    rows = [r for r in range(12) if r != 3]
+    for name, got in (("h", h), ("y", y)):
+        check(name, got[rows], tuple(v[rows] for v in ref[name]), dt, 12)
+    assert torch.equal(h[3], x[3])
+
+
 def test_nothing_to_do(cuda):
     x, t, pw, w, gv, _, _ = problem(cuda, torch.bfloat16, 0, 64, "channel")
     leaves = [v.requires_grad_() for v in (x, t, pw, w, gv)]
