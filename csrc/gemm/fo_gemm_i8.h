@@ -13,6 +13,7 @@ namespace fo {
 constexpr int kI8BK = 128;            // elements of K in one 128-byte swizzle atom
 constexpr int kI8MaxK = 131071;       // 128 * 128 * K stays below 2^31
 constexpr int kI8MaxExperts = 1024;
+constexpr int kI8MaxRows = INT32_MAX - 1023;  // of A and of a weight matrix: tiles that begin inside end below 2^31
 
 struct GemmI8Params {
   int M, N, K;

@@ -450,7 +450,7 @@ static void check_i8_weights(const at::Tensor& like, int64_t K, const at::Tensor
   const int64_t N = B.size(-2), E = grouped ? B.size(0) : 1;
   FO_CHECK(B.size(-1) == K, "the activations [..., K] and B disagree on K");
   FO_CHECK(K >= 16 && K % 16 == 0 && K <= kI8MaxK, "K must be a multiple of 16 from 16 to ", kI8MaxK, " (K=", K, ")");
-  FO_CHECK(N >= 8 && N % 8 == 0 && N <= INT32_MAX, "N must be a multiple of 8 (N=", N, ")");
+  FO_CHECK(N >= 8 && N % 8 == 0 && N <= kI8MaxRows, "N must be a multiple of 8 (N=", N, ")");
   FO_CHECK(SB.is_cuda() && SB.is_contiguous() && SB.scalar_type() == at::kFloat && SB.dim() == (grouped ? 2 : 1) &&
                SB.numel() == E * N && SB.size(-1) == N,
            grouped ? "SB must be a contiguous float32 CUDA tensor [experts, N]" : "SB must be a contiguous float32 CUDA tensor [N]");
@@ -501,7 +501,7 @@ void OverlapImpl::GemmI8(at::Tensor A, at::Tensor B, at::Tensor SA, at::Tensor S
   GemmI8Params p;
   check_i8_weights(A, A.size(1), B, SB, offsets, &p);
   const int64_t M = A.size(0);
-  FO_CHECK(M <= INT32_MAX, "too many rows");
+  FO_CHECK(M <= kI8MaxRows, "too many rows");
   FO_CHECK(SA.is_cuda() && SA.is_contiguous() && SA.scalar_type() == at::kFloat && SA.dim() == 1 && SA.size(0) == M,
            "SA must be a contiguous float32 CUDA tensor [M]");
   FO_CHECK(C.is_cuda() && C.is_contiguous() && (C.scalar_type() == at::kBFloat16 || C.scalar_type() == at::kHalf) &&
@@ -535,7 +535,7 @@ at::Tensor OverlapImpl::LinearI8(at::Tensor X, at::Tensor B, at::Tensor SB, c10:
   at::Tensor x = X.dim() == 2 && X.is_contiguous() ? X : X.reshape({-1, K}).contiguous();
   if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone();
   const int64_t M = x.size(0);
-  FO_CHECK(M <= INT32_MAX, "too many rows");
+  FO_CHECK(M <= kI8MaxRows, "too many rows");
   p.M = static_cast<int>(M);
   const bool bf16 = x.scalar_type() == at::kBFloat16;
   at::Tensor c = fresh({M, p.N}, x.scalar_type(), x);

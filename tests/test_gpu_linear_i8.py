@@ -214,6 +214,27 @@ def test_replayed_graph_and_another_stream(cuda, impl):
     impl.check_status()
 
 
+def test_beyond_32_bit_offsets(cuda, impl):
+    """C and the activations pass 2^31 elements, then the weights do."""
+    M, N, K = 270000, 8192, 64
+    x = torch.randn(M, K, device=cuda).to(torch.bfloat16)
+    _, b, _, sb = _operands(cuda, 1, N, K)
+    y = ops.linear_i8(impl, x, b, sb)
+    for lo in (0, M // 2, M - 700):
+        assert torch.equal(y[lo:lo + 700], ops.linear_i8(impl, x[lo:lo + 700], b, sb))
+    del x, y
+    experts, N, K = 40, 8192, 8192
+    b = torch.randint(-128, 128, (experts, N, K), device=cuda, dtype=torch.int8)
+    sb = torch.rand(experts, N, device=cuda) * 1e-2
+    for rows in (3, 300):                      # either kernel
+        x = torch.randn(2 * rows, K, device=cuda).to(torch.bfloat16)
+        offsets = torch.tensor([0] + [rows] * (experts - 1) + [2 * rows], device=cuda, dtype=torch.int32)
+        y = ops.linear_i8(impl, x, b, sb, offsets)
+        for e, part in ((0, slice(0, rows)), (experts - 1, slice(rows, 2 * rows))):
+            assert torch.equal(y[part], ops.linear_i8(impl, x[part], b[e], sb[e]))
+    impl.check_status()
+
+
 def test_refuses(cuda, impl):
     a, b, sa, sb = _operands(cuda, 32, 64, 128)
     c = torch.empty(32, 64, device=cuda, dtype=torch.bfloat16)

@@ -239,6 +239,23 @@ def test_replayed_graph_and_another_stream(cuda):
             assert torch.equal(a, b)
 
 
+def test_rows_beyond_32_bit_offsets(cuda):
+    """2.2e9 elements, each row as by itself; the weights' gradients of rows that are alike add up."""
+    dt, rows, dim = torch.bfloat16, 270000, 8192
+    x, t, pw, w, gv, gh, gy = problem(cuda, dt, 1000, dim, None)
+    far = [v.repeat(rows // 1000, 1) for v in (x, t, gh, gy)]
+    op = torch.ops.flashoverlap_op
+    h, y, stats = op.rmsnorm_add_rmsnorm(far[0], far[1], pw, w, None, 0.5, EPS, True)
+    h1, y1, stats1 = op.rmsnorm_add_rmsnorm(x, t, pw, w, None, 0.5, EPS, True)
+    assert torch.equal(h[-1000:], h1) and torch.equal(y[-1000:], y1) and torch.equal(h[:1000], h1)
+    grads = op.rmsnorm_add_rmsnorm_backward(far[2], far[3], far[0], far[1], pw, w, None, stats, 0.5)
+    alone = op.rmsnorm_add_rmsnorm_backward(gh, gy, x, t, pw, w, None, stats1, 0.5)
+    for a, b in zip(grads[:2], alone[:2]):
+        assert torch.equal(a[-1000:], b) and torch.equal(a[134000:135000], b)
+    for a, b in zip(grads[2:4], alone[2:4]):           # two roundings to bf16, and 32-bit sums of 270000 terms
+        assert ((a.double() - 270 * b.double()).norm() <= 2 * 2.0 ** -8 * (270 * b.double()).norm())
+
+
 def test_refuses(cuda):
     x, t, pw, w, gv, gh, gy = problem(cuda, torch.bfloat16, 24, 64, 4)
     for bad in ((x.cpu(), t, pw, w, gv), (x, t.cpu(), pw, w, gv), (x.float(), t.float(), pw.float(), w.float(), None), (x, t.half(), pw, w, gv),
