@@ -31,7 +31,8 @@ __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr)
 // expert in a row of its own in shared memory; the counts of the warps and, through distributed shared memory, of the CTAs in
 // front of it give each warp its first row for every expert, and a second walk over the same run hands the rows out, 32
 // choices a step: ballots over the expert's bits tell each lane which others have its expert (half the time of match.any, whose
-// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us with eight CTAs).  Bound by latency.
+// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us with eight CTAs).  Bound by latency:
+// 16 x 8 choices 5.2 us, 8192 x 8 of 64 9.6 us, 16384 x 8 of 256 14 us.
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     moe_sort_kernel(const Id* __restrict__ ids, int64_t n, int experts, int32_t* __restrict__ slot,
@@ -177,6 +178,7 @@ __device__ __forceinline__ void zero_rows(uint4* rows, int64_t first, int64_t la
 }
 
 // Bound by the rows written: every token's row is read once.  A thread copies one vector of a token to its top_k rows.
+// 8192 x 8 rows of 4096: 97 us (6.2 TB/s), 16384 x 2 of 8192: 124 us (6.5 TB/s).
 __global__ void __launch_bounds__(kRowThreads)
     moe_dispatch_kernel(const uint4* __restrict__ X, const int32_t* __restrict__ slot,
                         const int32_t* __restrict__ offsets, uint4* __restrict__ R, int tokens, int top_k, int nvec,
@@ -222,7 +224,8 @@ __device__ __forceinline__ void unpack8(const uint4& p, float2 (&f)[4]) {
 }
 
 // Bound by the rows read.  A thread sums VPT vectors of a token over its top_k rows, in their order; KC rows of them are in flight at
-// once, and where a token has few rows more of its vectors are.
+// once, and where a token has few rows more of its vectors are (one vector a thread: 16384 x 2 rows of 8192 in 316 us, now 145;
+// 8192 x 8 of 4096: 93 us, 6.5 TB/s).
 template <bool BF16, int KC, int VPT>
 __global__ void __launch_bounds__(kRowThreads)
     moe_combine_kernel(const uint4* __restrict__ R, const void* __restrict__ w, bool f32,
@@ -282,7 +285,8 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // Bound by memory: the token's gradient is read once, every row of the experts is read (for its weight's gradient) and its
-// gradient written.  A CTA takes a token; the dots are summed over its threads in a fixed order.
+// gradient written.  A CTA takes a token; the dots are summed over its threads in a fixed order.  8192 x 8 rows of 4096: 194 us
+// (5.9 TB/s), 16384 x 2 of 8192: 210 us (6.4 TB/s).
 template <bool BF16, int KC, int VPT, bool ROWS, bool WEIGHTS>
 __global__ void __launch_bounds__(kRowThreads)
     moe_combine_backward_kernel(const uint4* __restrict__ GO, const uint4* __restrict__ R, const void* __restrict__ w,
