@@ -16,6 +16,10 @@
 // expert by bisection.  A tile's rows past the expert's last one are multiplied (they are the next expert's)
 // and not stored.
 //
+// Kernels that follow one another closely (ptx::grid_wait) begin before their inputs are written, so no load of an input goes the
+// read-only way (ld.global.nc, which __ldg and const __restrict__ pointers are compiled to): it is for data that nobody writes while
+// the kernel exists.
+//
 // Every wait is bounded: on expiry the role records a status code, raises a CTA-wide abort flag, the producer drains its
 // TMA loads in flight, TMEM is freed and the kernel returns.
 #pragma once
@@ -28,7 +32,8 @@ namespace fo {
 
 // Rows [0, first) and [last, M) of C, zeroed by `threads` threads of which this is number `at`.
 __device__ __forceinline__ void i8_zero_outside(const GemmI8Params& p, int64_t at, int64_t threads) {
-  const int first = min(max(p.offsets[0], 0), p.M), last = min(max(p.offsets[p.experts], 0), p.M);
+  const int first = min(max(__ldca(p.offsets), 0), p.M);
+  const int last = min(max(__ldca(p.offsets + p.experts), 0), p.M);
   const int64_t nvec = p.N / 8;
   uint4* c = reinterpret_cast<uint4*>(p.C);
   const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -42,7 +47,7 @@ struct I8Segment {
   bool bad;
 };
 __device__ __forceinline__ I8Segment i8_segment(const GemmI8Params& p, int e) {
-  I8Segment s{p.offsets[e], p.offsets[e + 1], false};
+  I8Segment s{__ldca(p.offsets + e), __ldca(p.offsets + e + 1), false};
   if (s.lo < 0 || s.hi < s.lo || s.hi > p.M) {
     s.bad = true;
     s.hi = s.lo = 0;
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
   if constexpr (GROUPED) {
     for (int e = threadIdx.x; e < p.experts; e += kI8WideThreads) {
       const I8Segment s = i8_segment(p, e);
-      if (s.bad && blockIdx.x == 0) ptx::report_status(p.status, kStatusBadArgument, 3, e, p.offsets[e]);
+      if (s.bad && blockIdx.x == 0) ptx::report_status(p.status, kStatusBadArgument, 3, e, __ldca(p.offsets + e));
       s_first[e] = (s.hi - s.lo + kI8Rows - 1) / kI8Rows;
       s_rows[e] = s.lo;
     }
@@ -191,7 +196,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
       }
       w.expert = lo;
       w.row = s_rows[lo] + (tc.m - s_first[lo]) * kI8Rows + rank * 128;
-      w.row_end = p.offsets[lo + 1];
+      w.row_end = __ldca(p.offsets + lo + 1);
     } else {
       w.expert = 0;
       w.row = tc.m * kRows + rank * MT * 128;
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
       // whole rows of the warp leave by tensor store (which leaves out what lies beyond the matrix), an expert's last
       // ones by thread, since behind them are the next expert's
       const bool use_tma = !GROUPED || row0 + 32 <= work.row_end;
-      const float sa = row0 + lane < work.row_end ? __ldg(p.SA + row0 + lane) : 0.f;
+      const float sa = row0 + lane < work.row_end ? __ldca(p.SA + row0 + lane) : 0.f;
       const float* sb = p.SB + static_cast<size_t>(work.expert) * p.N + work.n0;
       ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(&tmem_full_bar[acc], acc_phase, s_abort, pipe_timeout));
       if (!ok) {
@@ -369,8 +374,8 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
           const int b = 8 * (j & 3);
           float s[8] = {};
           if (8 * j < cols) {  // N is a multiple of 8
-            const float4 s0 = __ldg(reinterpret_cast<const float4*>(sb + c * 64 + 8 * j));
-            const float4 s1 = __ldg(reinterpret_cast<const float4*>(sb + c * 64 + 8 * j + 4));
+            const float4 s0 = __ldca(reinterpret_cast<const float4*>(sb + c * 64 + 8 * j));
+            const float4 s1 = __ldca(reinterpret_cast<const float4*>(sb + c * 64 + 8 * j + 4));
             s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w;
             s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
           }
@@ -653,7 +658,7 @@ __global__ void __launch_bounds__(kI8NarrowThreads)
   if (ok && warp_idx >= 2) {
     // ------------------------------------------------------------------ epilogue, second half
     const int n = n0 + row;
-    const float sb = n < p.N ? __ldg(p.SB + static_cast<size_t>(expert) * p.N + n) : 0.f;
+    const float sb = n < p.N ? __ldca(p.SB + static_cast<size_t>(expert) * p.N + n) : 0.f;
 #pragma unroll 4
     for (int c = 0; c < kOwn; c += 4) {
       const int token = token0 + rank * kOwn + c;
@@ -672,7 +677,7 @@ __global__ void __launch_bounds__(kI8NarrowThreads)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (token + i < token_end && n < p.N) {
-          const float f = static_cast<float>(static_cast<int32_t>(v[i])) * __ldg(p.SA + token + i) * sb;
+          const float f = static_cast<float>(static_cast<int32_t>(v[i])) * __ldca(p.SA + token + i) * sb;
           p.C[static_cast<size_t>(token + i) * p.N + n] = to16<BF16>(f);
         }
       }

@@ -13,6 +13,10 @@ namespace fo {
 
 namespace {
 
+// Kernels that follow one another closely (ptx::grid_wait) begin before their inputs are written, so no load of an input goes the
+// read-only way (ld.global.nc, which __ldg and const __restrict__ pointers are compiled to): it is for data that nobody writes while
+// the kernel exists.
+
 // ---------------------------------------------------------------------------- the order
 
 constexpr int kSortThreads = 1024;
@@ -58,7 +62,7 @@ __global__ void __launch_bounds__(kSortThreads)
   // expert of choice i; `experts` for a choice without one and for lanes past the end
   auto expert_at = [&](int64_t i) -> int {
     if (i >= end) return experts;
-    const Id v = ids[i];
+    const Id v = __ldca(ids + i);
     return v >= 0 && v < static_cast<Id>(experts) ? static_cast<int>(v) : experts;
   };
   // the walks go in batches whose loads are in flight together
@@ -165,7 +169,7 @@ constexpr int kRowThreads = 256;
 // The row of a choice if it is one of the `rows` there are, else -1: an order made for something else is not followed
 // out of the matrix.
 __device__ __forceinline__ int row_at(const int32_t* slot, int64_t choice, int64_t rows) {
-  const int row = slot[choice];
+  const int row = __ldca(slot + choice);
   return static_cast<uint32_t>(row) < static_cast<uint32_t>(rows) ? row : -1;
 }
 
@@ -197,18 +201,15 @@ __global__ void __launch_bounds__(kRowThreads)
       if (row >= 0) R[static_cast<int64_t>(row) * nvec + j] = x;
     }
   }
-  zero_rows(R, offsets[experts], static_cast<int64_t>(tokens) * top_k, nvec);
+  zero_rows(R, __ldca(offsets + experts), static_cast<int64_t>(tokens) * top_k, nvec);
 }
 
 template <bool BF16>
 __device__ __forceinline__ float weight_at(const void* w, bool f32, int64_t i) {
   if (w == nullptr) return 1.f;
-  if (f32) return static_cast<const float*>(w)[i];
-  if constexpr (BF16) {
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
-  } else {
-    return __half2float(static_cast<const __half*>(w)[i]);
-  }
+  if (f32) return __ldca(static_cast<const float*>(w) + i);
+  const uint32_t bits = __ldca(static_cast<const unsigned short*>(w) + i);
+  return unpack2<BF16>(bits).x;
 }
 
 // The kernels that read a token's rows have a build for each number of rows that a thread requests at once; more choices
@@ -285,10 +286,10 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // Bound by memory: the token's gradient is read once, every row of the experts is read (for its weight's gradient) and its
-// gradient written.  A CTA takes a token; the dots are summed over its threads in a fixed order.  8192 x 8 rows of 4096: 194 us
-// (5.9 TB/s), 16384 x 2 of 8192: 210 us (6.4 TB/s).
+// gradient written.  A CTA takes a token, three of them an SM; the dots are summed over its threads in a fixed order.  8192 x 8 rows of 4096: 183 us
+// (6.2 TB/s; 194 with two an SM), 16384 x 2 of 8192: 215 us (6.2 TB/s).
 template <bool BF16, int KC, int VPT, bool ROWS, bool WEIGHTS>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 3)
     moe_combine_backward_kernel(const uint4* __restrict__ GO, const uint4* __restrict__ R, const void* __restrict__ w,
                                 bool f32, const int32_t* __restrict__ slot, const int32_t* __restrict__ offsets,
                                 uint4* __restrict__ DR, void* __restrict__ DW, int tokens, int top_k, int nvec,
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int j = j0 + i * blockDim.x;
-        if (j < nvec) g[i] = __ldg(GO + token * nvec + j);
+        if (j < nvec) g[i] = __ldca(GO + token * nvec + j);
       }
       if constexpr (WEIGHTS) {
 #pragma unroll
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kRowThreads)
       }
     }
   }
-  if constexpr (ROWS) zero_rows(DR, offsets[experts], rows, nvec);
+  if constexpr (ROWS) zero_rows(DR, __ldca(offsets + experts), rows, nvec);
 }
 
 template <typename Kernel, typename... Args>

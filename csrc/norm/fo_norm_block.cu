@@ -92,7 +92,10 @@ __device__ __forceinline__ float4 row_sums(const float4& v, float (*red)[128], i
                      __shfl_sync(0xffffffffu, t, 3));
 }
 
-__device__ __forceinline__ uint4 ld_vec(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+// Kernels that follow one another closely (ptx::grid_wait) begin before their inputs are written, so no load of an input goes the
+// read-only way (ld.global.nc, which __ldg and const __restrict__ pointers are compiled to): it is for data that nobody writes while
+// the kernel exists.
+__device__ __forceinline__ uint4 ld_vec(const uint16_t* p) { return __ldca(reinterpret_cast<const uint4*>(p)); }
 
 // The rows a thread reads come through a ring in shared memory that it fills with asynchronous copies, STAGES - 1 rows
 // ahead.  Every thread copies and reads words of its own only, so the ring needs no barrier, and the loads in
@@ -409,10 +412,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) norm_block_backward_kernel(con
       if constexpr (GATE == kRowGate) pw16[i] = ld_vec(p.PW + c.first + i * c.step);
     }
   }
-  float2 next_stats = row_begin < row_end ? __ldg(p.stats + row_begin) : f2(0.f);
+  float2 next_stats = row_begin < row_end ? __ldca(p.stats + row_begin) : f2(0.f);
   for (int b = row_begin; b < row_end; ++b) {
     const float2 r1 = f2(next_stats.x), r2 = f2(next_stats.y);
-    if (b + 1 < row_end) next_stats = __ldg(p.stats + b + 1);
+    if (b + 1 < row_end) next_stats = __ldca(p.stats + b + 1);
     const size_t row = static_cast<size_t>(b) * dim + c.first;
     ring.wait();
     // s0 = sum GY W n2.  With u = n1 G PW the other mean, sum b n1, is sum GH u + r2 (sum GY W u - s0 / dim sum n2 u): all
