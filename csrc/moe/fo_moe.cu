@@ -225,7 +225,7 @@ __device__ __forceinline__ void unpack8(const uint4& p, float2 (&f)[4]) {
 }
 
 // Bound by the rows read.  A thread sums VPT vectors of a token over its top_k rows, in their order; KC rows of them are in flight at
-// once, and where a token has few rows more of its vectors are (one vector a thread: 16384 x 2 rows of 8192 in 316 us, now 145;
+// once, and where a token has few rows more of its vectors are (one vector a thread: 16384 x 2 rows of 8192 in 316 us, now 130;
 // 8192 x 8 of 4096: 93 us, 6.5 TB/s).
 template <bool BF16, int KC, int VPT>
 __global__ void __launch_bounds__(kRowThreads)
@@ -439,7 +439,8 @@ bool valid(const MoeShape& s) {
 
 int64_t vec_ctas(const MoeShape& s) { return (static_cast<int64_t>(s.tokens) * (s.dim / 8) + kRowThreads - 1) / kRowThreads; }
 
-// Rows requested at once, and vectors of each, for a number of choices: about eight loads a thread.
+// Rows requested at once, and vectors of each, for a number of choices: about eight loads a thread, four where eight take the registers of
+// a third CTA an SM (two rows, four vectors each: 16384 x 2 rows of 8192 in 144 us, two vectors: 130).
 template <bool BF16, int KC, int VPT>
 cudaError_t launch_combine(const MoeShape& s, const uint4* r, MoeWeights w, const int32_t* slot, uint4* o, cudaStream_t stream) {
   const int nvec = s.dim / 8;
@@ -452,7 +453,7 @@ template <bool BF16>
 cudaError_t combine(const MoeShape& s, const uint4* r, MoeWeights w, const int32_t* slot, uint4* o, cudaStream_t stream) {
   switch (s.top_k) {
     case 1: return launch_combine<BF16, 1, 4>(s, r, w, slot, o, stream);
-    case 2: return launch_combine<BF16, 2, 4>(s, r, w, slot, o, stream);
+    case 2: return launch_combine<BF16, 2, 2>(s, r, w, slot, o, stream);
     case 3: return launch_combine<BF16, 3, 2>(s, r, w, slot, o, stream);
     case 4: return launch_combine<BF16, 4, 2>(s, r, w, slot, o, stream);
     case 5:
