@@ -192,7 +192,7 @@ GemmI8Plan choose_i8(int M, int N, int K, int experts, bool grouped) {
   }
   for (int tokens : {16, 32, 64, 128}) {
     for (int split : {1, 2, 4, 8}) {
-      if (4 * split > tokens || split * kI8BK > K) continue;  // sums are exchanged four tokens at a time
+      if (4 * split > tokens || (split > 1 && split * kI8BK > K)) continue;  // sums are exchanged four tokens at a time
       const double t = narrow_time(M, N, K, experts, grouped, tokens, split);
       if (t < best) {
         best = t;

@@ -145,6 +145,8 @@ int64_t OverlapImpl::GetOption(std::string name) {
   if (name == "last_algo") return last_algo_;
   if (name == "last_split") return last_split_;
   if (name == "last_tail") return last_tail_;
+  if (name == "last_i8_tokens") return last_i8_tokens_;
+  if (name == "last_i8_split") return last_i8_split_;
   if (name == "validate") return opt_validate_;
   if (name == "wait_sleep_ns") return opt_wait_sleep_ns_;
   if (name == "pull_direct") return opt_pull_direct_;
@@ -489,6 +491,8 @@ void OverlapImpl::run_i8(GemmI8Params* p, const void* A, const float* SA, const 
   p->status = status_.data_ptr<int>();
   p->timeout_ns = static_cast<uint64_t>(opt_timeout_ms_) * 1000000ull;
   const GemmI8Plan plan = choose_i8(p->M, p->N, p->K, p->experts, p->offsets != nullptr);
+  last_i8_tokens_ = plan.tokens;
+  last_i8_split_ = plan.split;
   const std::string e = gemm_i8_launch(plan, *p, A, B, bf16, stream());
   FO_CHECK(e.empty(), "gemm_i8: ", e, " (M=", p->M, " N=", p->N, " K=", p->K, " experts=", p->experts, ")");
 }

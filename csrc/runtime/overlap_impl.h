@@ -213,6 +213,8 @@ class OverlapImpl : public torch::CustomClassHolder {
   // What the last plain GEMM ran (read-only options last_algo, last_split, last_tail): the Algo whose
   // kernel, the CTAs of a split over K (0: none), and the scheduling units computed as halves.
   std::atomic<int> last_algo_{-1}, last_split_{0}, last_tail_{0};
+  // What the last 8-bit product ran (GemmI8Plan; read-only options last_i8_tokens, last_i8_split).
+  std::atomic<int> last_i8_tokens_{-1}, last_i8_split_{0};
   int64_t opt_exact_algo_ = 0;   // plain GEMM: 1 runs the Algo's own kernel even where another is faster
   int64_t opt_split_k_ = -1;     // plain GEMM of few tiles split over K: -1 automatic, 0 never, else that many CTAs a tile
   int64_t opt_tma_out_ = -1;     // plain kernels' stores: 0 per-thread stores, else TMA tensor stores where the output allows

@@ -102,6 +102,35 @@ def test_gemm(cuda, impl, dt, M, N, K):
     assert mem[0].isnan().all() and mem[-1].isnan().all()          # nothing beyond the matrix
 
 
+# a problem for everything that may run: tokens of a tile and split (0, 1: 256-row tiles; 0, 2: 512), M, N, K, experts (0: dense)
+PLANS = [(0, 1, 9929, 40, 48, 0), (0, 1, 9825, 40, 48, 2), (0, 2, 14245, 272, 18032, 0), (16, 1, 1, 40, 48, 0), (16, 1, 2, 40, 48, 1),
+         (16, 2, 2, 4264, 656, 0), (16, 2, 43, 40, 736, 40), (16, 4, 1, 40, 512, 0), (16, 4, 1, 40, 528, 1), (32, 1, 4924, 40, 48, 0), (32, 1, 4777, 40, 48, 1),
+         (32, 2, 2646, 40, 1264, 0), (32, 2, 2454, 48, 1168, 1), (32, 4, 1234, 40, 896, 0), (32, 4, 1333, 40, 848, 6), (32, 8, 1, 40, 1552, 0),
+         (32, 8, 1, 40, 1568, 1), (64, 1, 62, 13168, 16736, 0), (64, 1, 13468, 40, 144, 54), (64, 2, 4910, 40, 1600, 0), (64, 2, 4731, 40, 1616, 7),
+         (64, 4, 2399, 40, 1584, 0), (64, 4, 2648, 40, 1296, 2), (64, 8, 1252, 40, 2992, 0), (64, 8, 1225, 40, 2880, 1), (128, 1, 11218, 40, 3936, 0),
+         (128, 1, 9694, 40, 4320, 44), (128, 2, 4922, 40, 4432, 0), (128, 2, 5020, 40, 4976, 2), (128, 4, 2421, 48, 7280, 0), (128, 4, 2320, 40, 7920, 6),
+         (128, 8, 1247, 40, 15472, 0), (128, 8, 1150, 48, 12928, 5)]
+
+
+@pytest.mark.parametrize("tokens,split,M,N,K,experts", PLANS)
+def test_every_kernel(cuda, impl, tokens, split, M, N, K, experts):
+    a, b, sa, sb = _operands(cuda, M, N, K, experts)
+    mem = torch.full((M + 2, N), float("nan"), device=cuda, dtype=torch.bfloat16)
+    c = mem[1:M + 1]
+    if experts:                                    # uneven, the first one's none if there are others, two rows nobody's
+        cuts = (torch.linspace(0, 1, experts)[1:] ** 2 * max(M - 2, 1)).int().tolist() if experts > 1 else [max(M - 2, 1)]
+        offsets = torch.tensor([0, *([0] if experts > 1 else []), *cuts], device=cuda, dtype=torch.int32)
+        ref = torch.zeros(M, N, dtype=torch.float64, device=cuda)
+        for e, lo, hi in _segments(offsets, M):
+            ref[lo:hi] = _ref(a[lo:hi], b[e], sa[lo:hi], sb[e])
+    else:
+        offsets, ref = None, _ref(a, b, sa, sb)
+    impl.gemm_i8(a, b, sa, sb, c, offsets)
+    impl.check_status()
+    assert (impl.get_option("last_i8_tokens"), impl.get_option("last_i8_split")) == (tokens, split)
+    assert _close(c, ref, torch.bfloat16) and mem[0].isnan().all() and mem[-1].isnan().all()
+
+
 @pytest.mark.parametrize("M", [1, 40, 500])
 def test_gemm_largest_sums(cuda, impl, M):
     a, b, sa, sb = _operands(cuda, M, 256, 131056, extreme=True)

@@ -72,7 +72,9 @@ def problem(cuda, dt, rows, dim, gate, seed=0):
 
 # one vector, a part of a warp, every number of vectors a thread, its first and last sizes; one row, fewer and more than CTAs
 SHAPES = [(1, 8, None), (3, 8, 3), (130, 72, "channel"), (7, 2048, 7), (200, 2056, 2), (5000, 264, 8), (3000, 1024, 1500), (1200, 4104, "channel"),
-          (33, 8192, None), (600, 8200, 3), (12, 16384, "row"), (301, 16384, "channel"), (2, 4096, 2), (20000, 16, 4), (1, 16384, "channel")]
+          (33, 8192, None), (600, 8200, 3), (12, 16384, "row"), (301, 16384, "channel"), (2, 4096, 2), (20000, 16, 4), (1, 16384, "channel"),
+          # lines that CTAs share: fewer lines than CTAs, more, and both for rows that a cluster shares; lines that are one CTA's
+          (1024, 8192, 64), (1600, 8192, 200), (9000, 1032, 900), (600, 9000, 30), (1000, 16384, 125), (2072, 8192, 148)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
