@@ -199,6 +199,35 @@ def test_linear(cuda, impl, dt, shape, N):
     assert _close(y.reshape(-1, N), _ref(q.to(cuda), b, s.to(cuda), sb), dt)
 
 
+# a token or a few, every split; K that ends inside a block or a 16-byte piece of it; one row more, and longer rows
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("N,K", [(8, 16), (40, 48), (136, 144), (4096, 528), (1024, 1040), (28672, 1024), (136, 2064), (8192, 3584), (4096, 4112), (40, 8192), (40, 8208)])
+def test_linear_of_a_few_tokens_is_its_two_steps(cuda, impl, dt, N, K):
+    _, b, _, sb = _operands(cuda, 1, N, K)
+    for M in (1, 2, 3, 4, 5):
+        x = (torch.randn(M, K, device=cuda) * torch.logspace(-2, 2, M, device=cuda)[:, None]).to(dt)
+        x[0, -1] = 100.0                           # the largest lies in the last CTA's part
+        if M == 3:
+            x[1, 0] = float("inf")
+            x[2] = 0
+        mem = torch.full((M, N), float("nan"), device=cuda, dtype=dt)
+        q, s = ops.quantize_rows(x)
+        impl.gemm_i8(q, b, s, sb, mem, None)
+        y = ops.linear_i8(impl, x, b, sb)
+        impl.check_status()
+        assert torch.equal(y.view(torch.int16), mem.view(torch.int16)) or (M == 3 and torch.equal(y[[0, 2]], mem[[0, 2]]) and y[1].isnan().all())
+        if M == 1:                                 # in a graph, behind a kernel that lets it start early
+            graph, w = torch.cuda.CUDAGraph(), torch.ones(K, device=cuda, dtype=dt)
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                n = ops.rmsnorm(x, w)
+                captured = ops.linear_i8(impl, n, b, sb)
+            for _ in range(3):
+                x.normal_()
+                graph.replay()
+                assert torch.equal(captured, ops.linear_i8(impl, ops.rmsnorm(x, w), b, sb))
+
+
 def test_linear_special_rows_stay_in_their_rows(cuda, impl):
     x = torch.randn(20, 64, device=cuda).to(torch.bfloat16)
     x[3, 1], x[7, 5], x[11] = float("nan"), float("inf"), 0
