@@ -253,7 +253,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm_a
     *to = dense(g);
   }
   FO_CHECK(stats.is_cuda() && stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.dim() == 2 &&
-               stats.size(0) == X.size(0) && stats.size(1) == 2,
+               stats.size(0) == X.size(0) && stats.size(1) == 2 && reinterpret_cast<uintptr_t>(stats.data_ptr()) % 8 == 0,
            "stats must be what the forward pass returned");
   fo::check_device(stats, X, "stats");
   const at::ScalarType type = o.X.scalar_type();

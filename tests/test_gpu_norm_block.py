@@ -274,3 +274,10 @@ def test_refuses(cuda):
     for a, b, s in ((gh.half(), gy, stats), (gh[:12], gy, stats), (gh, gy.cpu(), stats), (gh, gy, stats[:12]), (gh, gy, stats.double()), (gh, gy, stats.cpu())):
         with pytest.raises(RuntimeError):
             op.rmsnorm_add_rmsnorm_backward(a, b, x, t, pw, w, gv, s, 1.0)
+
+
+def test_refuses_stats_between_words(cuda):
+    x, t, pw, w, gv, gh, gy = problem(cuda, torch.bfloat16, 24, 64, 4)
+    odd = torch.zeros(49, device=cuda)[1:].view(24, 2)   # pairs that do not lie on 8 bytes
+    with pytest.raises(RuntimeError, match="stats"):
+        torch.ops.flashoverlap_op.rmsnorm_add_rmsnorm_backward(gh, gy, x, t, pw, w, gv, odd, 1.0)
