@@ -188,7 +188,7 @@ NormBlockOperands norm_block_operands(const at::Tensor& X, const at::Tensor& T, 
   FO_CHECK(X.dim() == 2 && T.sizes() == X.sizes(), "X and T must be [rows, dim]");
   const int64_t rows = X.size(0), dim = X.size(1);
   FO_CHECK(dim >= 8 && dim % 8 == 0 && dim <= 16384, "dim must be a multiple of 8 from 8 to 16384 (", dim, ")");
-  FO_CHECK(rows <= INT32_MAX, "too many rows");
+  FO_CHECK(rows <= fo::kMaxNormBlockRows, "too many rows");
   FO_CHECK(PW.dim() == 1 && PW.size(0) == dim && W.dim() == 1 && W.size(0) == dim, "PW and W must be [dim]");
   int64_t lines = 1;
   if (given(G)) {

@@ -715,7 +715,7 @@ Gate gate_of(const NormBlock& p) {
 }
 
 bool valid(const NormBlock& p) {
-  return p.dim >= 8 && p.dim % 8 == 0 && p.dim <= kMaxDim && p.rows >= 1 && p.lines >= 1 && p.rows % p.lines == 0;
+  return p.dim >= 8 && p.dim % 8 == 0 && p.dim <= kMaxDim && p.rows >= 1 && p.rows <= kMaxNormBlockRows && p.lines >= 1 && p.rows % p.lines == 0;
 }
 
 }  // namespace

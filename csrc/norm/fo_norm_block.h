@@ -3,7 +3,11 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cstdint>
+
 namespace fo {
+
+constexpr int kMaxNormBlockRows = INT32_MAX - 3;  // the number of a row that is loaded three ahead stays an int
 
 // One call's operands: 16-bit row-major [rows, dim], weights [dim], gate [lines, dim] (lines consecutive groups of
 // rows / lines rows share a line; nullptr: no gate), stats [rows][2] fp32 = (r1, r2).

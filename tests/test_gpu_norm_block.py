@@ -281,3 +281,11 @@ def test_refuses_stats_between_words(cuda):
     odd = torch.zeros(49, device=cuda)[1:].view(24, 2)   # pairs that do not lie on 8 bytes
     with pytest.raises(RuntimeError, match="stats"):
         torch.ops.flashoverlap_op.rmsnorm_add_rmsnorm_backward(gh, gy, x, t, pw, w, gv, odd, 1.0)
+
+
+def test_refuses_rows_whose_numbers_do_not_fit(cuda):
+    x, w = torch.zeros(1, 8, device=cuda, dtype=torch.bfloat16), torch.ones(8, device=cuda, dtype=torch.bfloat16)
+    for rows in (2 ** 31 - 3, 2 ** 31 - 1, 2 ** 31):
+        many = x.expand(rows, 8)
+        with pytest.raises(RuntimeError, match="too many rows"):
+            ops.rmsnorm_add_rmsnorm(many, many, w, w)
