@@ -153,9 +153,16 @@ void check_leaf_in_capture(const at::Tensor& t) {
            "release that graph (its loss and outputs) before the capture");
 }
 
+// Forward-mode derivatives do not exist either, and would get lost without a word.
+template <typename... T>
+void check_no_tangent(const T&... t) {
+  FO_CHECK(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), "this operator has no forward-mode derivative");
+}
+
 // Whether a call has a gradient to record.
 template <typename... T>
 bool records(const T&... t) {
+  check_no_tangent(t...);
   if (!at::GradMode::is_enabled() || !((t.defined() && t.requires_grad()) || ...)) return false;
   if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) (check_leaf_in_capture(t), ...);
   return true;
@@ -163,6 +170,7 @@ bool records(const T&... t) {
 
 template <typename... T>
 void check_no_gradient(const char* what, const T&... t) {
+  check_no_tangent(t...);
   FO_CHECK(!at::GradMode::is_enabled() || !(t.requires_grad() || ...), what, " has no gradient: call it under no_grad, or detach its inputs");
 }
 

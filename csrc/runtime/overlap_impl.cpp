@@ -529,6 +529,7 @@ at::Tensor OverlapImpl::LinearI8(at::Tensor X, at::Tensor B, at::Tensor SB, c10:
   NvtxRange nvtx_range("flashoverlap::linear_i8");
   FO_CHECK(!at::GradMode::is_enabled() || !(X.requires_grad() || SB.requires_grad()),
            "linear_i8 has no gradient: call it under no_grad, or detach its inputs");
+  FO_CHECK(!X._fw_grad(/*level=*/0).defined() && !SB._fw_grad(/*level=*/0).defined(), "linear_i8 has no forward-mode derivative");
   FO_CHECK(X.is_cuda() && (X.scalar_type() == at::kBFloat16 || X.scalar_type() == at::kHalf) && X.dim() >= 1,
            "X must be a bfloat16 or float16 CUDA tensor [..., K]");
   GemmI8Params p;

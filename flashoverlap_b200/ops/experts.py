@@ -14,7 +14,10 @@ from ._native import native
 
 
 class ExpertOrder(NamedTuple):
-    """Rows of ``tokens * top_k`` choices sorted by expert, an expert's in the order of their tokens."""
+    """Rows of ``tokens * top_k`` choices sorted by expert, an expert's in the order of their tokens.
+
+    As ``moe_sort`` returns it.  To drop a choice (an expert's capacity, padding) set its id to -1 and sort: a -1 written into
+    ``slot`` afterwards leaves its row among the expert's, with nothing in it."""
     slot: torch.Tensor      # [tokens, top_k] int32: the row of every choice, -1 for one that is not served here
     source: torch.Tensor    # [tokens * top_k] int32: the choice (token * top_k + k) of every row, -1 behind the last
     offsets: torch.Tensor   # [experts + 1] int32: every expert's first row; the last entry is the number of rows

@@ -192,3 +192,42 @@ def test_8_bit_objects_are_made_before_a_capture(cuda):
     fresh.gemm_i8(a, a, s, s, c, None)
     fresh.check_status()
     assert (c == 0).all()
+
+
+def test_other_derivatives_are_refused_not_lost(cuda):
+    """Forward-mode derivatives raise, and what torch.func makes of the operators is right or raises; nothing comes back without
+    its derivative."""
+    import torch.autograd.forward_ad as fwd
+    impl = ops.OverlapImpl()
+    impl.nccl_init(0, 1, [0] * 16)
+    x, t = (torch.randn(8, 64, device=cuda).bfloat16() for _ in range(2))
+    w, sb = torch.ones(64, device=cuda).bfloat16(), torch.ones(64, device=cuda)
+    b = torch.ones(64, 64, device=cuda, dtype=torch.int8)
+    order = ops.moe_sort(torch.zeros(8, 2, dtype=torch.int32, device=cuda), 4)
+    calls = (lambda a: ops.rmsnorm_add_rmsnorm(a, t, w, w)[1], lambda a: ops.rmsnorm_add_rmsnorm(x, a, w, w, w)[0],
+             lambda a: ops.moe_dispatch(a, order), lambda a: ops.moe_combine(torch.cat([a, a]), None, order),
+             lambda a: ops.quantize_rows(a)[1], lambda a: ops.linear_i8(impl, a, b, sb))
+    for f in calls:
+        with fwd.dual_level():
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    f(fwd.make_dual(x, x))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (x,))
+        try:
+            each = torch.func.vmap(f)(torch.stack([x, t]))
+        except RuntimeError:
+            pass
+        else:
+            assert torch.equal(each, torch.stack([f(x), f(t)]))
+        try:
+            grad = torch.func.grad(lambda v: f(v).float().sum())(x)
+        except RuntimeError:
+            pass
+        else:
+            v = x.detach().requires_grad_()
+            f(v).float().sum().backward()
+            assert torch.equal(grad, v.grad)
+    weights = torch.rand(8, 2, device=cuda)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        ops.moe_combine(torch.cat([x, x]), fwd.make_dual(weights, weights), order)
