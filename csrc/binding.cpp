@@ -352,6 +352,24 @@ fo::MoeShape moe_shape(const at::Tensor& like, int64_t dim, const at::Tensor& sl
   return s;
 }
 
+// What tells which rows no slot names: the order's sources if they are of its choices, else (or beyond them) a scratch.
+struct MoeSourceTensors {
+  at::Tensor source, scratch;
+  fo::MoeSources arg() const {
+    return {source.defined() ? source.data_ptr<int>() : nullptr, scratch.defined() ? scratch.data_ptr<int>() : nullptr};
+  }
+};
+MoeSourceTensors moe_sources(const fo::MoeShape& s, const c10::optional<at::Tensor>& source, const at::Tensor& slot) {
+  MoeSourceTensors t;
+  if (given(source) && source->device() == slot.device() && source->scalar_type() == at::kInt && source->is_contiguous() &&
+      source->numel() == slot.numel()) {
+    t.source = *source;
+  }
+  const int64_t words = fo::moe_scratch_words(s, t.source.defined());
+  if (words > 0) t.scratch = fo::fresh({words}, at::kInt, slot);
+  return t;
+}
+
 // The router's weights, contiguous; none: undefined.
 at::Tensor moe_weights(const c10::optional<at::Tensor>& weights, const at::Tensor& like, const at::Tensor& slot) {
   if (!given(weights)) return {};
@@ -365,8 +383,8 @@ fo::MoeWeights weights_arg(const at::Tensor& w) {
   return w.defined() ? fo::MoeWeights{w.data_ptr(), w.scalar_type() == at::kFloat} : fo::MoeWeights{nullptr, false};
 }
 
-// R [tokens * top_k, dim]: R[slot[t, k]] = X[t], the rows behind the last expert's zero.
-at::Tensor dispatch_rows(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
+// R [tokens * top_k, dim]: R[slot[t, k]] = X[t], every other row zero.
+at::Tensor dispatch_rows(at::Tensor X, at::Tensor slot, at::Tensor offsets, const c10::optional<at::Tensor>& source) {
   check_16bit(X, "X");
   FO_CHECK(X.dim() == 2 && slot.dim() == 2 && X.size(0) == slot.size(0), "X must be [tokens, dim] and slot [tokens, top_k]");
   c10::cuda::CUDAGuard guard(X.device());
@@ -374,7 +392,8 @@ at::Tensor dispatch_rows(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
   const at::Tensor x = dense(X);
   at::Tensor R = fo::fresh({slot.numel(), X.size(1)}, X.scalar_type(), X);
   if (s.tokens > 0) {
-    fo::cuda_check(fo::moe_dispatch_launch(s, x.data_ptr(), slot.data_ptr<int>(), offsets.data_ptr<int>(), R.data_ptr(),
+    const MoeSourceTensors from = moe_sources(s, source, slot);
+    fo::cuda_check(fo::moe_dispatch_launch(s, x.data_ptr(), slot.data_ptr<int>(), offsets.data_ptr<int>(), from.arg(), R.data_ptr(),
                                            c10::cuda::getCurrentCUDAStream().stream()),
                    "moe_dispatch");
   }
@@ -400,7 +419,8 @@ at::Tensor combine_rows(at::Tensor R, c10::optional<at::Tensor> weights, at::Ten
 // (gradient of R, gradient of weights) from that of O; one that is not asked for comes back empty.
 std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::optional<at::Tensor> R,
                                                         c10::optional<at::Tensor> weights, at::Tensor slot,
-                                                        at::Tensor offsets, bool for_rows, bool for_weights) {
+                                                        at::Tensor offsets, bool for_rows, bool for_weights,
+                                                        c10::optional<at::Tensor> source) {
   check_16bit(GO, "GO");
   FO_CHECK(GO.dim() == 2 && slot.dim() == 2 && GO.size(0) == slot.size(0), "GO must be [tokens, dim] and slot [tokens, top_k]");
   FO_CHECK(for_rows || for_weights, "no gradient is asked for");
@@ -418,8 +438,9 @@ std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::opti
   DR = fo::fresh({for_rows ? slot.numel() : 0, GO.size(1)}, GO.scalar_type(), GO);
   DW = for_weights ? fo::fresh(slot.sizes(), w.scalar_type(), GO) : fo::fresh({0}, GO.scalar_type(), GO);
   if (s.tokens > 0) {
+    const MoeSourceTensors from = for_rows ? moe_sources(s, source, slot) : MoeSourceTensors{};
     fo::cuda_check(fo::moe_combine_backward_launch(s, go.data_ptr(), r.defined() ? r.data_ptr() : nullptr, weights_arg(w),
-                                                   slot.data_ptr<int>(), offsets.data_ptr<int>(),
+                                                   slot.data_ptr<int>(), offsets.data_ptr<int>(), from.arg(),
                                                    for_rows ? DR.data_ptr() : nullptr, for_weights ? DW.data_ptr() : nullptr,
                                                    c10::cuda::getCurrentCUDAStream().stream()),
                    "moe_combine_backward");
@@ -428,45 +449,46 @@ std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::opti
 }
 
 struct DispatchFunction : public torch::autograd::Function<DispatchFunction> {
-  static at::Tensor forward(AutogradContext* ctx, at::Tensor X, at::Tensor slot, at::Tensor offsets) {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor X, at::Tensor slot, at::Tensor offsets, c10::optional<at::Tensor> source) {
     ctx->save_for_backward({slot});
-    return dispatch_rows(X, slot, offsets);
+    return dispatch_rows(X, slot, offsets, source);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list v = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView below;
-    return once("moe_dispatch", {combine_rows(grads[0], c10::nullopt, v[0], nullptr), at::Tensor(), at::Tensor()});
+    return once("moe_dispatch", {combine_rows(grads[0], c10::nullopt, v[0], nullptr), at::Tensor(), at::Tensor(), at::Tensor()});
   }
 };
 
-at::Tensor moe_dispatch(at::Tensor X, at::Tensor slot, at::Tensor offsets) {
-  return records(X) ? DispatchFunction::apply(X, slot, offsets) : dispatch_rows(X, slot, offsets);
+at::Tensor moe_dispatch(at::Tensor X, at::Tensor slot, at::Tensor offsets, c10::optional<at::Tensor> source) {
+  return records(X) ? DispatchFunction::apply(X, slot, offsets, source) : dispatch_rows(X, slot, offsets, source);
 }
 
 struct CombineFunction : public torch::autograd::Function<CombineFunction> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot,
-                            at::Tensor offsets) {
+                            at::Tensor offsets, c10::optional<at::Tensor> source) {
     const at::Tensor w = or_undefined(weights);
     // the rows are kept only for the weights' gradient
-    ctx->save_for_backward({w.defined() && w.requires_grad() ? R : at::Tensor(), w, slot, offsets});
+    ctx->save_for_backward({w.defined() && w.requires_grad() ? R : at::Tensor(), w, slot, offsets, or_undefined(source)});
     return combine_rows(R, weights, slot, &offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list v = ctx->get_saved_variables();
     const bool rows = ctx->needs_input_grad(0), weights = v[0].defined() && ctx->needs_input_grad(1);
-    variable_list out(4);
+    variable_list out(5);
     if (!rows && !weights) return out;
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [DR, DW] = moe_combine_backward(grads[0], or_none(v[0]), or_none(v[1]), v[2], v[3], rows, weights);
+    auto [DR, DW] = moe_combine_backward(grads[0], or_none(v[0]), or_none(v[1]), v[2], v[3], rows, weights, or_none(v[4]));
     if (rows) out[0] = DR;
     if (weights) out[1] = DW;
     return once("moe_combine", std::move(out));
   }
 };
 
-at::Tensor moe_combine(at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot, at::Tensor offsets) {
+at::Tensor moe_combine(at::Tensor R, c10::optional<at::Tensor> weights, at::Tensor slot, at::Tensor offsets,
+                       c10::optional<at::Tensor> source) {
   const at::Tensor w = or_undefined(weights);
-  return records(R, w) ? CombineFunction::apply(R, or_none(w), slot, offsets) : combine_rows(R, weights, slot, &offsets);
+  return records(R, w) ? CombineFunction::apply(R, or_none(w), slot, offsets, source) : combine_rows(R, weights, slot, &offsets);
 }
 
 // (Q int8, S fp32 [rows]) of X [rows, dim].
@@ -665,9 +687,11 @@ TORCH_LIBRARY(flashoverlap_op, m) {
   m.def("rmsnorm_add_rmsnorm", &rmsnorm_add_rmsnorm);
   m.def("rmsnorm_add_rmsnorm_backward", &rmsnorm_add_rmsnorm_backward);
   m.def("moe_sort", &moe_sort);
-  m.def("moe_dispatch", &moe_dispatch);
-  m.def("moe_combine", &moe_combine);
-  m.def("moe_combine_backward", &moe_combine_backward);
+  // (source: of the sort; without it the call finds out by itself which rows no slot names, with a launch more)
+  m.def("moe_dispatch(Tensor X, Tensor slot, Tensor offsets, Tensor? source=None) -> Tensor", &moe_dispatch);
+  m.def("moe_combine(Tensor R, Tensor? weights, Tensor slot, Tensor offsets, Tensor? source=None) -> Tensor", &moe_combine);
+  m.def("moe_combine_backward(Tensor GO, Tensor? R, Tensor? weights, Tensor slot, Tensor offsets, bool for_rows, bool for_weights, "
+        "Tensor? source=None) -> (Tensor, Tensor)", &moe_combine_backward);
   m.def("quantize_rows", &quantize_rows);
   m.def("reorder", &reorder);
   m.def("unreorder", &unreorder);

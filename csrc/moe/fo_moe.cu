@@ -173,35 +173,111 @@ __device__ __forceinline__ int row_at(const int32_t* slot, int64_t choice, int64
   return static_cast<uint32_t>(row) < static_cast<uint32_t>(rows) ? row : -1;
 }
 
-// The rows behind the last expert's, zeroed by all threads of the grid.
+// The rows that belong to experts, as far as the matrix has them.
+__device__ __forceinline__ int64_t served_rows(const int32_t* offsets, int experts, int64_t rows) {
+  return min(max(static_cast<int64_t>(__ldca(offsets + experts)), static_cast<int64_t>(0)), rows);
+}
+
+// Rows [first, last), zeroed by all threads of the grid.
 __device__ __forceinline__ void zero_rows(uint4* rows, int64_t first, int64_t last, int nvec) {
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const int64_t end = last * nvec;
-  for (int64_t v = max(first, static_cast<int64_t>(0)) * nvec + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < end; v += step) rows[v] = zero;
+  for (int64_t v = first * nvec + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < end; v += step) rows[v] = zero;
+}
+
+// Rows below `served` that no slot names, zeroed: the row of a choice whose slot was set to -1 in a sorted order.  A thread looks
+// after a row, which is named if the choice that back[row] holds names it; so are all rows of a sorted order with its own
+// sources.  Where it does not, nobody names the row if `back` is the scratch of moe_inverse_kernel (`exact`), but sources may
+// also be of something else: then the CTA goes through all slots.  8192 x 8 rows of 512: 13.0 us sorted (12.8 without any of this),
+// 33 with a tenth dropped; with a scratch 14.3 and 14.6, but one launch more also for the host, which waits for 16 x 8 rows (13.8 us a
+// sort and dispatch either way).  So the scratch is made where a call brings no sources, and for more than kNamedScan choices,
+// since the search's cost grows with their square (8192 x 8 rows of 4096: 96, 106 with a tenth dropped, and 98 with a scratch).
+constexpr int64_t kNamedScan = 65536;
+
+struct NamedRows {
+  const int32_t* back;
+  bool exact;
+};
+
+// The row that this thread looks after first.
+__device__ __forceinline__ int64_t first_own_row() { return static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; }
+
+// All threads of the grid call this.  `back`: of first_own_row(), fetched ahead (whatever it is where there is no such row).
+__device__ __forceinline__ void zero_unnamed_rows(uint4* R, const int32_t* slot, const NamedRows& n, int32_t back, int64_t served,
+                                                  int64_t choices, int nvec) {
+  __shared__ uint32_t named[kRowThreads / 32];  // a bit for each row of the CTA
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t own = first_own_row(); own - threadIdx.x < served; own += step) {
+    if (own >= step) back = own < served ? __ldca(n.back + own) : -1;
+    const bool there = own < served;
+    const bool is = there && static_cast<uint32_t>(back) < static_cast<uint32_t>(choices) && __ldca(slot + back) == own;
+    uint32_t left = __ballot_sync(0xffffffffu, there && !is);
+    if (!n.exact && __syncthreads_or(left)) {
+      constexpr int kAhead = 8;  // loads in flight
+      const int first = static_cast<int>(own - threadIdx.x), last = static_cast<int>(choices);  // kNamedScan at most
+      if (lane == 0) named[warp] = 0;
+      __syncthreads();
+#pragma unroll 1
+      for (int c0 = threadIdx.x; c0 < last; c0 += kAhead * blockDim.x) {
+        uint32_t r[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int c = c0 + u * static_cast<int>(blockDim.x);
+          r[u] = c < last ? static_cast<uint32_t>(__ldca(slot + c)) - first : 0xffffffffu;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (r[u] < blockDim.x) atomicOr(&named[r[u] >> 5], 1u << (r[u] & 31));
+        }
+      }
+      __syncthreads();
+      left &= ~named[warp];
+      __syncthreads();  // the bits have been read
+    }
+    for (; left != 0; left &= left - 1) {
+      uint4* row = R + (own - lane + __ffs(left) - 1) * nvec;
+      for (int j = lane; j < nvec; j += 32) row[j] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// inverse[slot[c]] = c.  Rows that no slot names keep what was there, which the look back tells.
+__global__ void __launch_bounds__(kRowThreads)
+    moe_inverse_kernel(const int32_t* __restrict__ slot, int32_t* __restrict__ inverse, int64_t choices) {
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+  ptx::grid_launch_dependents();
+  ptx::grid_wait();
+  if (c >= choices) return;
+  const int row = row_at(slot, c, choices);
+  if (row >= 0) inverse[row] = static_cast<int32_t>(c);
 }
 
 // Bound by the rows written: every token's row is read once.  A thread copies one vector of a token to its top_k rows.
 // 8192 x 8 rows of 4096: 97 us (6.2 TB/s), 16384 x 2 of 8192: 124 us (6.5 TB/s).
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 8)
     moe_dispatch_kernel(const uint4* __restrict__ X, const int32_t* __restrict__ slot,
-                        const int32_t* __restrict__ offsets, uint4* __restrict__ R, int tokens, int top_k, int nvec,
-                        int experts) {
+                        const int32_t* __restrict__ offsets, NamedRows named, uint4* __restrict__ R,
+                        int tokens, int top_k, int nvec, int experts) {
   const int64_t v = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
   ptx::grid_launch_dependents();
   ptx::grid_wait();
   const int64_t token = v / nvec;
+  const int64_t rows = static_cast<int64_t>(tokens) * top_k;
+  const int64_t served = served_rows(offsets, experts, rows);
+  const int32_t back = first_own_row() < rows ? __ldca(named.back + first_own_row()) : -1;
   if (token < tokens) {
     const int j = static_cast<int>(v - token * nvec);
     const uint4 x = __ldcs(X + v);
-    const int64_t rows = static_cast<int64_t>(tokens) * top_k;
 #pragma unroll 4
     for (int k = 0; k < top_k; ++k) {
-      const int row = row_at(slot, token * top_k + k, rows);
+      const int row = row_at(slot, token * top_k + k, served);
       if (row >= 0) R[static_cast<int64_t>(row) * nvec + j] = x;
     }
   }
-  zero_rows(R, __ldca(offsets + experts), static_cast<int64_t>(tokens) * top_k, nvec);
+  zero_unnamed_rows(R, slot, named, back, served, rows, nvec);
+  zero_rows(R, served, rows, nvec);
 }
 
 template <bool BF16>
@@ -292,7 +368,7 @@ template <bool BF16, int KC, int VPT, bool ROWS, bool WEIGHTS>
 __global__ void __launch_bounds__(kRowThreads, 3)
     moe_combine_backward_kernel(const uint4* __restrict__ GO, const uint4* __restrict__ R, const void* __restrict__ w,
                                 bool f32, const int32_t* __restrict__ slot, const int32_t* __restrict__ offsets,
-                                uint4* __restrict__ DR, void* __restrict__ DW, int tokens, int top_k, int nvec,
+                                NamedRows named, uint4* __restrict__ DR, void* __restrict__ DW, int tokens, int top_k, int nvec,
                                 int experts) {
   __shared__ float part[kRowThreads / 32][KC];
   const int64_t token = blockIdx.x;
@@ -300,6 +376,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::grid_launch_dependents();
   ptx::grid_wait();
+  [[maybe_unused]] const int64_t served = ROWS ? served_rows(offsets, experts, rows) : 0;
   for (int k0 = 0; k0 < top_k; k0 += KC) {
     int row[KC];
     float wk[KC], dot[KC];
@@ -343,6 +420,7 @@ __global__ void __launch_bounds__(kRowThreads, 3)
             for (int n = 0; n < 4; ++n) dot[k] += gf[n].x * f[n].x + gf[n].y * f[n].y;
           }
           if constexpr (ROWS) {
+            if (row[k] >= served) continue;
             __stcs(DR + static_cast<int64_t>(row[k]) * nvec + j,
                    make_uint4(pack2<BF16>(wk[k] * gf[0].x, wk[k] * gf[0].y), pack2<BF16>(wk[k] * gf[1].x, wk[k] * gf[1].y),
                               pack2<BF16>(wk[k] * gf[2].x, wk[k] * gf[2].y), pack2<BF16>(wk[k] * gf[3].x, wk[k] * gf[3].y)));
@@ -377,7 +455,11 @@ __global__ void __launch_bounds__(kRowThreads, 3)
       }
     }
   }
-  if constexpr (ROWS) zero_rows(DR, __ldca(offsets + experts), rows, nvec);
+  if constexpr (ROWS) {
+    const int32_t back = first_own_row() < rows ? __ldca(named.back + first_own_row()) : -1;
+    zero_unnamed_rows(DR, slot, named, back, served, rows, nvec);
+    zero_rows(DR, served, rows, nvec);
+  }
 }
 
 template <typename Kernel, typename... Args>
@@ -437,6 +519,14 @@ bool valid(const MoeShape& s) {
          s.experts <= kMaxExperts && static_cast<int64_t>(s.tokens) * s.top_k <= INT32_MAX;
 }
 
+// How the rows that are named are told, made on the way if it takes the scratch.
+cudaError_t named_rows(const MoeShape& s, const int32_t* slot, const MoeSources& from, NamedRows* n, cudaStream_t stream) {
+  const int64_t choices = static_cast<int64_t>(s.tokens) * s.top_k;
+  *n = NamedRows{from.scratch != nullptr ? from.scratch : from.source, from.scratch != nullptr};
+  if (from.scratch == nullptr) return moe_scratch_words(s, from.source != nullptr) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+  return launch(moe_inverse_kernel, (choices + kRowThreads - 1) / kRowThreads, kRowThreads, stream, slot, from.scratch, choices);
+}
+
 int64_t vec_ctas(const MoeShape& s) { return (static_cast<int64_t>(s.tokens) * (s.dim / 8) + kRowThreads - 1) / kRowThreads; }
 
 // Rows requested at once, and vectors of each, for a number of choices: about eight loads a thread, four where eight take the registers of
@@ -467,6 +557,7 @@ struct BackwardCall {
   const uint4 *go, *r;
   MoeWeights w;
   const int32_t *slot, *offsets;
+  NamedRows named;
   uint4* dr;
   void* dw;
 };
@@ -478,7 +569,7 @@ cudaError_t launch_backward(const BackwardCall& c, cudaStream_t stream) {
   auto kernel = c.dr == nullptr   ? moe_combine_backward_kernel<BF16, KC, VPT, false, true>
                 : c.dw == nullptr ? moe_combine_backward_kernel<BF16, KC, VPT, true, false>
                                   : moe_combine_backward_kernel<BF16, KC, VPT, true, true>;
-  return launch(kernel, c.s.tokens, threads, stream, c.go, c.r, c.w.p, c.w.f32, c.slot, c.offsets, c.dr, c.dw, c.s.tokens,
+  return launch(kernel, c.s.tokens, threads, stream, c.go, c.r, c.w.p, c.w.f32, c.slot, c.offsets, c.named, c.dr, c.dw, c.s.tokens,
                 c.s.top_k, nvec, c.s.experts);
 }
 
@@ -497,6 +588,11 @@ cudaError_t backward(const BackwardCall& c, cudaStream_t stream) {
 
 }  // namespace
 
+int64_t moe_scratch_words(const MoeShape& s, bool sources) {
+  const int64_t choices = static_cast<int64_t>(s.tokens) * s.top_k;
+  return sources && choices <= kNamedScan ? 0 : choices;
+}
+
 cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int experts, int32_t* slot, int32_t* source,
                             int32_t* offsets, cudaStream_t stream) {
   if (experts < 1 || experts > kMaxExperts || choices < 0 || choices > INT32_MAX) return cudaErrorInvalidValue;
@@ -504,11 +600,14 @@ cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int ex
                : launch_sort<int32_t>(ids, choices, experts, slot, source, offsets, stream);
 }
 
-cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t* slot, const int32_t* offsets, void* R,
-                                cudaStream_t stream) {
+cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t* slot, const int32_t* offsets,
+                                const MoeSources& from, void* R, cudaStream_t stream) {
   if (!valid(s)) return cudaErrorInvalidValue;
+  NamedRows named;
+  const cudaError_t e = named_rows(s, slot, from, &named, stream);
+  if (e != cudaSuccess) return e;
   return launch(moe_dispatch_kernel, vec_ctas(s), kRowThreads, stream, static_cast<const uint4*>(X), slot, offsets,
-                static_cast<uint4*>(R), s.tokens, s.top_k, s.dim / 8, s.experts);
+                named, static_cast<uint4*>(R), s.tokens, s.top_k, s.dim / 8, s.experts);
 }
 
 cudaError_t moe_combine_launch(const MoeShape& s, const void* R, MoeWeights w, const int32_t* slot, void* O,
@@ -519,10 +618,15 @@ cudaError_t moe_combine_launch(const MoeShape& s, const void* R, MoeWeights w, c
 }
 
 cudaError_t moe_combine_backward_launch(const MoeShape& s, const void* GO, const void* R, MoeWeights w,
-                                        const int32_t* slot, const int32_t* offsets, void* DR, void* DW,
-                                        cudaStream_t stream) {
+                                        const int32_t* slot, const int32_t* offsets, const MoeSources& from, void* DR,
+                                        void* DW, cudaStream_t stream) {
   if (!valid(s) || (DR == nullptr && DW == nullptr)) return cudaErrorInvalidValue;
-  const BackwardCall c{s, static_cast<const uint4*>(GO), static_cast<const uint4*>(R), w, slot, offsets, static_cast<uint4*>(DR), DW};
+  NamedRows named{};
+  if (DR != nullptr) {
+    const cudaError_t e = named_rows(s, slot, from, &named, stream);
+    if (e != cudaSuccess) return e;
+  }
+  const BackwardCall c{s, static_cast<const uint4*>(GO), static_cast<const uint4*>(R), w, slot, offsets, named, static_cast<uint4*>(DR), DW};
   return s.bf16 ? backward<true>(c, stream) : backward<false>(c, stream);
 }
 

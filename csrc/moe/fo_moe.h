@@ -28,16 +28,24 @@ struct MoeShape {
   bool bf16;
 };
 
-// R[slot[t, k]] = X[t]; rows from offsets[experts] on: zero.
-cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t* slot, const int32_t* offsets, void* R,
-                                cudaStream_t stream);
+// What tells the two calls below which rows no slot names (they are zeros in what is written): the sort's `source`, or `scratch`
+// of moe_scratch_words int32 whatever it holds, where that is not 0.  The slots decide, not the sources: those save the search.
+struct MoeSources {
+  const int32_t* source;
+  int32_t* scratch;
+};
+int64_t moe_scratch_words(const MoeShape& s, bool sources);
+
+// R[slot[t, k]] = X[t]; every other row, and those from offsets[experts] on: zero.
+cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t* slot, const int32_t* offsets,
+                                const MoeSources& from, void* R, cudaStream_t stream);
 // O[t] = sum over k of w[t, k] * R[slot[t, k]] (w.p == nullptr: 1), choices without a row left out.
 cudaError_t moe_combine_launch(const MoeShape& s, const void* R, MoeWeights w, const int32_t* slot, void* O,
                                cudaStream_t stream);
-// DR[slot[t, k]] = w[t, k] * GO[t], rows from offsets[experts] on: zero; DW[t, k] = <GO[t], R[slot[t, k]]>, 0 without a row,
-// in w's type.  DR or DW may be nullptr.
+// DR[slot[t, k]] = w[t, k] * GO[t]; every other row, and those from offsets[experts] on: zero; DW[t, k] = <GO[t], R[slot[t, k]]>,
+// 0 without a row, in w's type.  DR (then `from` is not used) or DW may be nullptr.
 cudaError_t moe_combine_backward_launch(const MoeShape& s, const void* GO, const void* R, MoeWeights w,
-                                        const int32_t* slot, const int32_t* offsets, void* DR, void* DW,
-                                        cudaStream_t stream);
+                                        const int32_t* slot, const int32_t* offsets, const MoeSources& from, void* DR,
+                                        void* DW, cudaStream_t stream);
 
 }  // namespace fo

@@ -17,7 +17,8 @@ class ExpertOrder(NamedTuple):
     """Rows of ``tokens * top_k`` choices sorted by expert, an expert's in the order of their tokens.
 
     As ``moe_sort`` returns it.  To drop a choice (an expert's capacity, padding) set its id to -1 and sort: a -1 written into
-    ``slot`` afterwards leaves its row among the expert's, with nothing in it."""
+    ``slot`` afterwards leaves its row among the expert's, as a row of zeros.  An order made by hand
+    has no row twice among its slots and none from ``offsets[-1]`` on; its slots decide, and ``source`` may be None (a launch more)."""
     slot: torch.Tensor      # [tokens, top_k] int32: the row of every choice, -1 for one that is not served here
     source: torch.Tensor    # [tokens * top_k] int32: the choice (token * top_k + k) of every row, -1 behind the last
     offsets: torch.Tensor   # [experts + 1] int32: every expert's first row; the last entry is the number of rows
@@ -32,10 +33,10 @@ def moe_sort(ids: torch.Tensor, experts: int) -> ExpertOrder:
 
 
 def moe_dispatch(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
-    """The rows of ``x`` [tokens, dim] in the order: [tokens * top_k, dim], rows behind the last choice zero.
+    """The rows of ``x`` [tokens, dim] in the order: [tokens * top_k, dim], rows that no choice has are zero.
 
     bf16 or fp16, ``dim`` a multiple of 8.  The gradient of a token is the fp32 sum of its rows', rounded once."""
-    return native("moe_dispatch")(x, order[0], order[2])
+    return native("moe_dispatch")(x, order[0], order[2], order[1])
 
 
 def moe_combine(y: torch.Tensor, weights: Optional[torch.Tensor], order: ExpertOrder) -> torch.Tensor:
@@ -44,4 +45,4 @@ def moe_combine(y: torch.Tensor, weights: Optional[torch.Tensor], order: ExpertO
     ``y`` [tokens * top_k, dim] in bf16 or fp16, ``dim`` a multiple of 8; ``weights`` [tokens, top_k] in fp32 or ``y``'s
     type, or None for 1.  Sums are fp32, in the order of the choices, rounded once.  The gradient of a row without a choice
     and of a weight without a row is zero."""
-    return native("moe_combine")(y, weights, order[0], order[2])
+    return native("moe_combine")(y, weights, order[0], order[2], order[1])

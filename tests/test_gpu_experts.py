@@ -195,6 +195,83 @@ def test_an_order_of_something_else_stays_inside_the_matrix(cuda):
     assert ((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -20).all()
 
 
+def _poison(shape, dt, cuda):
+    """What the allocator hands out next holds NaN (a row number that is none, read as one)."""
+    kept = [torch.full(shape, float("nan"), device=cuda, dtype=dt) for _ in range(4)]
+    torch.cuda.synchronize()
+    del kept
+
+
+def _rows_ref(values, order, rows):
+    """[rows, dim]: ``values`` [tokens, top_k, dim] at the slots that lie in [0, offsets[-1]), zeros elsewhere."""
+    slot, last = order.slot.long(), min(max(int(order.offsets[-1]), 0), rows)
+    there = (slot >= 0) & (slot < last)
+    ref = torch.zeros(rows, values.shape[-1], dtype=values.dtype, device=values.device)
+    ref[slot[there]] = values[there]
+    return ref
+
+
+# one row, a part of what a warp looks after, every size on both sides of 65536 choices, rows of one vector (few warps for many rows)
+EDITED = [(1, 1, 1, 8), (3, 2, 2, 64), (128, 8, 16, 264), (205, 5, 7, 1032), (1100, 64, 300, 8), (8192, 8, 64, 72), (8193, 8, 64, 72), (700, 64, 1000, 2056),
+          (20000, 9, 33, 8)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("tokens,top_k,experts,dim", EDITED)
+@pytest.mark.parametrize("edit", ["dropped", "one", "all", "moved"])
+def test_rows_that_an_edited_order_leaves_out_are_zeros(cuda, dt, tokens, top_k, experts, dim, edit):
+    """Choices dropped from a sorted order by a -1 in their slots, or rows dealt out anew: a row that no slot names is zeros in the
+    dispatch's result and in the gradient of the combine's rows."""
+    order, x, y, w = _problem(cuda, dt, tokens, top_k, experts, dim)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    rows, last = tokens * top_k, int(order.offsets[-1])
+    slot = order.slot.clone()
+    if edit == "dropped":
+        slot[torch.rand(slot.shape, device=cuda, generator=g) < 0.3] = -1
+    elif edit == "one":
+        slot[slot == last // 2] = -1
+    elif edit == "all":
+        slot[:] = -1
+    else:                                          # other rows than the sort's, whose sources are then others too
+        to = torch.cat([torch.randperm(last, device=cuda, generator=g), torch.full((1,), -1, device=cuda)])
+        slot = to[slot.long()].to(torch.int32)
+        slot[::2, 0] = -1
+    order = order._replace(slot=slot)
+    # the sort's sources, which tell most, none, some that cannot be taken
+    for order in (order, order._replace(source=None), order._replace(source=order.source.long())):
+        _poison((rows, dim), dt, cuda)
+        assert torch.equal(ops.moe_dispatch(x, order), _rows_ref(x[:, None].expand(-1, top_k, -1), order, rows))
+        go = torch.randn(tokens, dim, device=cuda, generator=g).to(dt)
+        y.requires_grad_()
+        _poison((rows, dim), dt, cuda)
+        gy, = torch.autograd.grad(ops.moe_combine(y, w, order), y, go)
+        assert torch.equal(gy, _rows_ref((go.float()[:, None] * w[..., None]).to(dt), order, rows))
+        y.requires_grad_(False)
+        _poison((rows, dim), dt, cuda)
+        dr, dw = torch.ops.flashoverlap_op.moe_combine_backward(go, y, w, order.slot, order.offsets, True, True)
+        assert torch.equal(dr, gy) and (dw[order.slot < 0] == 0).all()
+
+
+@pytest.mark.parametrize("tokens,top_k", [(20, 2), (9000, 8)])
+def test_an_order_of_something_else_in_both_directions(cuda, tokens, top_k):
+    """Slots outside the matrix and offsets outside it: rows with a choice have its token, all others are zeros."""
+    order, x, y, w = _problem(cuda, torch.bfloat16, tokens, top_k, 4, 64)
+    n = tokens * top_k
+    slot = torch.where(order.slot == 3, 1 << 30, torch.where(order.slot == 5, -7, order.slot))
+    slot = torch.where(order.slot == 8, n, slot).to(torch.int32)
+    kept = (slot >= 0) & (slot < n)
+    go = torch.randn(tokens, 64, device=cuda).bfloat16()
+    for shift in (0, -3, -(1 << 20), 1 << 30):     # the last ones' rows are not the experts', nobody's are, all are
+        bad = order._replace(slot=slot, offsets=order.offsets + shift)
+        _poison((n, 64), torch.bfloat16, cuda)
+        assert torch.equal(ops.moe_dispatch(x, bad), _rows_ref(x[:, None].expand(-1, top_k, -1), bad, n))
+        _poison((n, 64), torch.bfloat16, cuda)
+        dr, dw = torch.ops.flashoverlap_op.moe_combine_backward(go, y, w, bad.slot, bad.offsets, True, True)
+        assert torch.equal(dr, _rows_ref((go.float()[:, None] * w[..., None]).bfloat16(), bad, n))
+        terms = go.double()[:, None] * y.double()[torch.where(kept, slot, 0).long()] * kept[..., None]
+        assert ((dw.double() - terms.sum(-1)).abs() <= 65 * 2.0 ** -24 * terms.abs().sum(-1)).all() and (dw[~kept] == 0).all()
+
+
 def test_rows_beyond_32_bit_offsets(cuda):
     """2.6e9 elements: byte and element offsets pass 32 bits."""
     tokens, top_k, dim = 40000, 8, 8192
