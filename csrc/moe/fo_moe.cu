@@ -102,9 +102,10 @@ __global__ void __launch_bounds__(kSortThreads)
       all += v;
     }
   }
-  // nobody reads another CTA's counts from here on
+  // Nobody reads another CTA's counts from here on.  The release form: a CTA without choices waits at the kernel's end only, and
+  // must not leave while a load of its counts is under way.
   __syncwarp();
-  if (ctas > 1) ptx::cluster_arrive_relaxed();
+  if (ctas > 1) ptx::cluster_arrive_release();
   // exclusive sums over the experts
   uint32_t incl = all;
 #pragma unroll

@@ -56,3 +56,19 @@ def test_a_tile_is_stamped_as_signalled_before_its_owners_can_see_it():
     code = _code("fo_gemm_sm100.cuh")
     loop = code[code.index("const int g = s_sig_g[slot]"):code.index("mbar_arrive(&sig_empty_bar[slot])")]
     assert loop.index("kTraceSignalled") < loop.index("red_relaxed_sys_add")
+
+
+CSRC = GEMM.parent
+
+
+@pytest.mark.parametrize("path,accesses", [("moe/fo_moe.cu", ["= ld_shared_cluster_u32("]),
+                                           ("norm/fo_norm_block.cu", ["ptx::st_shared_cluster_u32("])])
+def test_a_cluster_barrier_behind_remote_accesses_releases(path, accesses):
+    """A CTA may leave once the cluster has arrived: an arrive in its relaxed form does not wait for the accesses to another CTA's
+    shared memory in front of it, so the first arrive behind such an access is the release form."""
+    code = re.sub(r"//[^\n]*", "", (CSRC / path).read_text())
+    for access in accesses:
+        places = [m.end() for m in re.finditer(re.escape(access), code)]
+        assert places
+        for at in places:
+            assert re.search(r"cluster_arrive_(\w+)", code[at:]).group(1) == "release", code[at:at + 300]
