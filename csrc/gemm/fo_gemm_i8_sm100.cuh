@@ -420,8 +420,9 @@ __global__ void __launch_bounds__(kI8WideThreads, 1)
   __syncwarp();  // lanes that drained join theirs: the barriers' aligned forms take whole warps
   ptx::tc_fence_before_sync();
   // Neither CTA may free TMEM or leave while the other can still signal its barriers or its MMAs read this CTA's
-  // shared memory.  Execution order only: no data crosses here.
-  ptx::cluster_arrive_relaxed();
+  // shared memory.  The release form: the leader waits for nobody's hand-back of its last accumulators, whose signals have
+  // to arrive before it leaves.
+  ptx::cluster_arrive_release();
   ptx::cluster_wait_acquire();
   if (warp_idx == 1) {
     ptx::tc_fence_after_sync();

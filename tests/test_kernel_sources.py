@@ -62,7 +62,8 @@ CSRC = GEMM.parent
 
 
 @pytest.mark.parametrize("path,accesses", [("moe/fo_moe.cu", ["= ld_shared_cluster_u32("]),
-                                           ("norm/fo_norm_block.cu", ["ptx::st_shared_cluster_u32("])])
+                                           ("norm/fo_norm_block.cu", ["ptx::st_shared_cluster_u32("]),
+                                           ("gemm/fo_gemm_i8_sm100.cuh", ["ptx::mbar_arrive_cluster_tmem(", "ptx::st_shared_cluster_v4(", "ptx::st_shared_cluster_u32("])])
 def test_a_cluster_barrier_behind_remote_accesses_releases(path, accesses):
     """A CTA may leave once the cluster has arrived: an arrive in its relaxed form does not wait for the accesses to another CTA's
     shared memory in front of it, so the first arrive behind such an access is the release form."""
