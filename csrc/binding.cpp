@@ -316,18 +316,19 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rmsnorm_add_rmsnorm(at::Tensor X,
 }
 
 // (slot [tokens, top_k], source [tokens * top_k], offsets [experts + 1]) of the experts `ids` [tokens, top_k] chosen for each token.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_sort(at::Tensor ids, int64_t experts) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> moe_sort(at::Tensor ids, int64_t experts, int64_t most_ctas) {
   FO_CHECK(ids.is_cuda() && ids.dim() == 2 && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
            "ids must be an int32 or int64 CUDA tensor [tokens, top_k]");
   FO_CHECK(experts >= 1 && experts <= fo::kMaxExperts, "experts must be from 1 to ", fo::kMaxExperts, " (", experts, ")");
   FO_CHECK(ids.size(1) >= 1 && ids.size(1) <= fo::kMaxTopK, "top_k must be from 1 to ", fo::kMaxTopK, " (", ids.size(1), ")");
   FO_CHECK(ids.numel() <= INT32_MAX, "too many choices");
+  FO_CHECK(most_ctas >= 1 && most_ctas <= 16, "most_ctas must be from 1 to 16 (", most_ctas, ")");
   c10::cuda::CUDAGuard guard(ids.device());
   const at::Tensor c = ids.contiguous();
   at::Tensor slot = fo::fresh(ids.sizes(), at::kInt, ids), source = fo::fresh({ids.numel()}, at::kInt, ids);
   at::Tensor offsets = fo::fresh({experts + 1}, at::kInt, ids);
   fo::cuda_check(fo::moe_sort_launch(c.data_ptr(), c.scalar_type() == at::kLong, c.numel(), static_cast<int>(experts),
-                                     slot.data_ptr<int>(), source.data_ptr<int>(), offsets.data_ptr<int>(),
+                                     static_cast<int>(most_ctas), slot.data_ptr<int>(), source.data_ptr<int>(), offsets.data_ptr<int>(),
                                      c10::cuda::getCurrentCUDAStream().stream()),
                  "moe_sort");
   return {slot, source, offsets};
@@ -686,7 +687,8 @@ TORCH_LIBRARY(flashoverlap_op, m) {
   m.def("swiglu", &swiglu);
   m.def("rmsnorm_add_rmsnorm", &rmsnorm_add_rmsnorm);
   m.def("rmsnorm_add_rmsnorm_backward", &rmsnorm_add_rmsnorm_backward);
-  m.def("moe_sort", &moe_sort);
+  m.def("moe_sort(Tensor ids, int experts, int most_ctas=16) -> (Tensor, Tensor, Tensor)", &moe_sort);
+  m.def("moe_sort_ctas", [](int64_t choices, int64_t most) { return static_cast<int64_t>(fo::moe_sort_ctas(choices, static_cast<int>(most))); });
   // (source: of the sort; without it the call finds out by itself which rows no slot names, with a launch more)
   m.def("moe_dispatch(Tensor X, Tensor slot, Tensor offsets, Tensor? source=None) -> Tensor", &moe_dispatch);
   m.def("moe_combine(Tensor R, Tensor? weights, Tensor slot, Tensor offsets, Tensor? source=None) -> Tensor", &moe_combine);

@@ -480,29 +480,13 @@ cudaError_t launch(Kernel kernel, int64_t grid, int threads, cudaStream_t stream
   return e;
 }
 
-template <typename Id>
-cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, int32_t* source, int32_t* offsets,
-                        cudaStream_t stream) {
-  auto kernel = moe_sort_kernel<Id>;
-  const int smem = (kSortWarps + 2) * experts * static_cast<int>(sizeof(uint32_t));
-  static bool set[16] = {};  // the same whoever sets it
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 16 || !set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (kSortWarps + 2) * kMaxExperts * static_cast<int>(sizeof(uint32_t)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 16) set[dev] = true;
-  }
-  const int ctas = n <= kSortOne ? 1 : (n <= kSortEight ? 8 : 16);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+cudaLaunchConfig_t sort_config(int ctas, int smem, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, 1, 1);
   cfg.blockDim = dim3(kSortThreads, 1, 1);
@@ -510,7 +494,53 @@ cudaError_t launch_sort(const void* ids, int64_t n, int experts, int32_t* slot, 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const Id*>(ids), n, experts, slot, source, offsets);
+  return cfg;
+}
+
+// The largest cluster of the sort that the current device has a place for, and the kernel's attributes set on the way: sixteen
+// CTAs are more than every device or part of one (a partition, a context of fewer SMs) grants.
+template <typename Id>
+cudaError_t largest_sort(int* ctas) {
+  static int cache[16] = {};  // 0: not asked yet; the same whoever sets it
+  constexpr int smem = (kSortWarps + 2) * kMaxExperts * static_cast<int>(sizeof(uint32_t));
+  auto kernel = moe_sort_kernel<Id>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 16 && cache[dev] != 0) {
+    *ctas = cache[dev];
+    return cudaSuccess;
+  }
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  int most = 1;
+  for (int size : {16, 8}) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = sort_config(size, smem, nullptr, attr);
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0) {
+      most = size;
+      break;
+    }
+    cudaGetLastError();
+  }
+  if (dev < 16) cache[dev] = most;
+  *ctas = most;
+  return cudaSuccess;
+}
+
+template <typename Id>
+cudaError_t launch_sort(const void* ids, int64_t n, int experts, int most_ctas, int32_t* slot, int32_t* source,
+                        int32_t* offsets, cudaStream_t stream) {
+  int largest = 1;
+  cudaError_t e = largest_sort<Id>(&largest);
+  if (e != cudaSuccess) return e;
+  const int smem = (kSortWarps + 2) * experts * static_cast<int>(sizeof(uint32_t));
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = sort_config(moe_sort_ctas(n, std::min(most_ctas, largest)), smem, stream, attr);
+  e = cudaLaunchKernelEx(&cfg, moe_sort_kernel<Id>, static_cast<const Id*>(ids), n, experts, slot, source, offsets);
   if (e != cudaSuccess) cudaGetLastError();
   return e;
 }
@@ -594,11 +624,16 @@ int64_t moe_scratch_words(const MoeShape& s, bool sources) {
   return sources && choices <= kNamedScan ? 0 : choices;
 }
 
-cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int experts, int32_t* slot, int32_t* source,
-                            int32_t* offsets, cudaStream_t stream) {
-  if (experts < 1 || experts > kMaxExperts || choices < 0 || choices > INT32_MAX) return cudaErrorInvalidValue;
-  return ids64 ? launch_sort<int64_t>(ids, choices, experts, slot, source, offsets, stream)
-               : launch_sort<int32_t>(ids, choices, experts, slot, source, offsets, stream);
+int moe_sort_ctas(int64_t choices, int most) {
+  const int wanted = choices <= kSortOne ? 1 : (choices <= kSortEight ? 8 : 16);
+  return wanted <= most ? wanted : (wanted == 16 && most >= 8 ? 8 : 1);
+}
+
+cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int experts, int most_ctas, int32_t* slot,
+                            int32_t* source, int32_t* offsets, cudaStream_t stream) {
+  if (experts < 1 || experts > kMaxExperts || choices < 0 || choices > INT32_MAX || most_ctas < 1) return cudaErrorInvalidValue;
+  return ids64 ? launch_sort<int64_t>(ids, choices, experts, most_ctas, slot, source, offsets, stream)
+               : launch_sort<int32_t>(ids, choices, experts, most_ctas, slot, source, offsets, stream);
 }
 
 cudaError_t moe_dispatch_launch(const MoeShape& s, const void* X, const int32_t* slot, const int32_t* offsets,

@@ -12,9 +12,11 @@ constexpr int kMaxTopK = 64;
 // ids [tokens * top_k] (int32, or int64 with ids64): the experts chosen for each token, in [0, experts); any other
 // value is a choice that this GPU does not serve.  slot [tokens * top_k]: the row of each choice, -1 if not served;
 // source [tokens * top_k]: the choice of each row, -1 behind the last row; offsets [experts + 1]: each expert's first row.
-// Rows of an expert keep the order of their choices.
-cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int experts, int32_t* slot, int32_t* source,
-                            int32_t* offsets, cudaStream_t stream);
+// Rows of an expert keep the order of their choices.  The sort is one cluster of at most `most_ctas` CTAs, of 16, 8 or 1.
+cudaError_t moe_sort_launch(const void* ids, bool ids64, int64_t choices, int experts, int most_ctas, int32_t* slot,
+                            int32_t* source, int32_t* offsets, cudaStream_t stream);
+// The cluster that sorts that many choices where clusters of `most` CTAs have a place.
+int moe_sort_ctas(int64_t choices, int most);
 
 // The router's weights or their gradients: fp32, or the rows' 16-bit type.
 struct MoeWeights {

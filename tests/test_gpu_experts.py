@@ -52,6 +52,19 @@ def test_sort(cuda, tokens, top_k, experts, kind):
         assert torch.equal(a.cpu(), b)
 
 
+@pytest.mark.parametrize("tokens,top_k,experts", [(33, 1, 1024), (513, 8, 5), (700, 64, 1000), (40000, 8, 256)])
+def test_sort_in_smaller_clusters(cuda, tokens, top_k, experts):
+    """As on a device, or a part of one, without a place for a cluster of sixteen, or of eight."""
+    ids = torch.randint(-1, experts + 2, (tokens, top_k), device=cuda)
+    ref = ops.moe_sort(ids, experts)
+    for most in (15, 8, 7, 1):
+        for a, b in zip(torch.ops.flashoverlap_op.moe_sort(ids, experts, most), ref):
+            assert torch.equal(a, b)
+    for bad in (0, 17):
+        with pytest.raises(RuntimeError):
+            torch.ops.flashoverlap_op.moe_sort(ids, experts, bad)
+
+
 def test_sort_extremes(cuda):
     none = ops.moe_sort(torch.full((50, 4), -1, device=cuda), 9)
     assert (none.slot == -1).all() and (none.source == -1).all() and (none.offsets == 0).all()
