@@ -21,8 +21,10 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-// Choices up to which one CTA sorts, and eight; sixteen from there on.
-constexpr int kSortOne = 512, kSortEight = 8192;
+// Choices up to which one CTA sorts, and eight; sixteen from there on.  1, 8 and 16 CTAs, in us, back to back in a graph: 1024 choices of 64
+// experts 3.8, 4.6, 4.9; 2048 of 256 4.8, 5.1, 5.6; 4096 of 64 5.7, 4.8, 5.1; 8192 of 64 9.1, 4.8, 5.1; 12288 of 64 12.4, 5.6, 5.2; 65536
+// of 64 56, 10.2, 7.1.
+constexpr int kSortOne = 2048, kSortEight = 8192;
 constexpr int kSortBatch = 4;
 
 __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {

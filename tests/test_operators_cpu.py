@@ -32,6 +32,6 @@ def test_sorts_where_large_clusters_have_no_place(lib):
     """Sixteen CTAs for many choices, but never a cluster that the device cannot place."""
     ctas = torch.ops.flashoverlap_op.moe_sort_ctas
     for most in range(1, 17):
-        for choices in (0, 1, 512, 513, 8192, 8193, 2 ** 31 - 1):
-            wanted = 1 if choices <= 512 else 8 if choices <= 8192 else 16
+        for choices in (0, 1, 2048, 2049, 8192, 8193, 2 ** 31 - 1):
+            wanted = 1 if choices <= 2048 else 8 if choices <= 8192 else 16
             assert ctas(choices, most) == max(c for c in (1, 8, 16) if c <= min(most, wanted))
