@@ -193,6 +193,84 @@ def test_values_that_only_their_norm_brings_into_range(cuda):
     assert torch.equal(h[3], x[3])
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,dim,gate", [(1, 64, "channel"), (40, 1032, "channel"), (20, 8192, "channel"), (5, 9000, "channel"), (40, 1032, "row"),
+                                           (64, 256, 4), (40, 1032, None), (12, 9000, "row")])
+def test_gradients_of_rows_whose_parts_cancel(cuda, dt, rows, dim, gate):
+    """H is what is left of roundings in every second row, and 1 / rms of it large: gradients within what 32 bits leave of H."""
+    x, t, pw, w, gv, gh, gy = problem(cuda, dt, rows, dim, gate)
+    u = reference(torch.zeros_like(x), t, pw, w, gv, 1.0)["h"][0]
+    x[::2] = (-u / 0.7).to(dt)[::2]
+    inputs = (x, t, pw, w, gv)
+    names = ["x", "t", "pw", "w"] + (["gate"] if gv is not None else [])
+    leaves = [v.requires_grad_() for v in inputs if v is not None]
+    h, y = ops.rmsnorm_add_rmsnorm(*inputs, 0.7, EPS)
+    detached = [None if v is None else v.detach() for v in inputs]
+    xd, td, pwd, wd = (v.double() for v in detached[:4])
+    lines = 1 if gv is None else gv.numel() // dim
+    g = torch.ones(1, dim, dtype=torch.float64, device=cuda) if gv is None else detached[4].double().view(lines, dim)
+    g = g.repeat_interleave(rows // lines, 0)
+    mean = lambda v: v.mean(1, keepdim=True)
+    r1 = 1 / (mean(td * td) + EPS).sqrt()
+    n1, pg = td * r1, pwd * g
+    hd, hm = 0.7 * xd + n1 * pg, (0.7 * xd).abs() + (n1 * pg).abs()
+    r2 = 1 / (mean(hd * hd) + EPS).sqrt()
+    n2 = hd * r2
+    few = 2.0 ** -16                               # of what is added up, as in check()
+    for a_gh, a_gy in ((gh, gy), (None, gy), (gh, None)):
+        outs, grads = zip(*[(o, v) for o, v in ((h, a_gh), (y, a_gy)) if v is not None])
+        got = dict(zip(names, torch.autograd.grad(outs, leaves, grads, retain_graph=True)))
+        ref = reference(*detached, 0.7, a_gh, a_gy)
+        zero = torch.zeros_like(xd)
+        ghd, gyd = (zero if v is None else v.double() for v in (a_gh, a_gy))
+        a = (gyd * wd).abs()
+        # H is off by `few` of its parts, its mean square by twice the mean of |H| times that, so 1 / rms relatively by
+        # few * rms(parts) / rms(H), and n2 = H / rms by both
+        off_r2 = few * mean(hm * hm).sqrt() * r2
+        off_n2 = few * hm * r2 + n2.abs() * off_r2
+        # dH = gh + r2 (a - n2 mean(a n2)): every factor's error times the others
+        c2 = mean(a * n2.abs())
+        off_c2 = mean(a * off_n2) + few * c2
+        off_dh = few * ghd.abs() + (few + off_r2) * r2 * (a + n2.abs() * c2) + r2 * (off_n2 * c2 + n2.abs() * off_c2)
+        dh = ref["x"][0] / 0.7
+        # the second mean, of dH G PW n1, is made of sums of dH's parts: those errors once for dH and once for the sums
+        off_c1 = 2 * mean(off_dh * (n1 * pg).abs())
+        b = (dh * pg).abs()
+        off_t = r1 * (off_dh * pg.abs() + n1.abs() * off_c1 + few * (b + n1.abs() * mean(b * n1.abs())))
+        column = few + rows * 2.0 ** -24           # and a column's sum has up to `rows` terms
+        off = {"x": 0.7 * off_dh, "t": off_t, "w": (gyd.abs() * off_n2 + column * (gyd * n2).abs()).sum(0),
+               "pw": ((off_dh + column * dh.abs()) * (g * n1).abs()).sum(0)}
+        if gv is not None:
+            off["gate"] = ((off_dh + column * dh.abs()) * (pwd * n1).abs()).view(lines, rows // lines, dim).sum(1).view(gv.shape)
+        for name, v in got.items():
+            value = ref[name][0]
+            assert ((v.double() - value).abs() <= half_step(dt) * value.abs() + 1.01 * off[name] + smallest(dt)).all(), (
+                name, float(((v.double() - value).abs() - half_step(dt) * value.abs()).max()), float(off[name].max()))
+            # The bound would see a term that is missing or has the wrong sign.  (What is left in H is about 2^-9 (bf16) or 2^-12 (fp16) of
+            # its parts, of which 2^-16 are 2^-7 or 2^-4 of H; each gradient has that in from two to four factors.)
+            assert float(off[name].norm()) <= 0.5 * float(value.norm())
+
+
+@pytest.mark.parametrize("gate", ["channel", "row"])
+def test_gradients_of_values_that_only_their_norm_brings_into_range(cuda, gate):
+    dt = torch.bfloat16
+    x, t, pw, w, gv, gh, gy = problem(cuda, dt, 12, 2048, gate)
+    t, gv = t * 1e16, gv * 3e3
+    t[3], t[4] = t[3] * 1e20, 0
+    leaves = [v.requires_grad_() for v in (x, t, pw, w, gv)]
+    got = torch.autograd.grad(ops.rmsnorm_add_rmsnorm(*leaves, 1.0, EPS), leaves, (gh, gy))
+    detached = [v.detach().clone() for v in leaves]
+    detached[1][3] = 0                             # squares beyond 32 bits: as in the forward pass, nothing is left of the row's block
+    ref = reference(*detached, 1.0, gh, gy)
+    rows = [r for r in range(12) if r != 3]
+    for name, v in zip(("x", "t", "pw", "w", "gate"), got):
+        if name == "t":
+            assert (v[3] == 0).all()
+            check(name, v[rows], tuple(u[rows] for u in ref[name]), dt, 12)
+        else:
+            check(name, v, ref[name], dt, 12)
+
+
 def test_nothing_to_do(cuda):
     x, t, pw, w, gv, _, _ = problem(cuda, torch.bfloat16, 0, 64, "channel")
     leaves = [v.requires_grad_() for v in (x, t, pw, w, gv)]
