@@ -520,7 +520,9 @@ __global__ void __launch_bounds__(kI8NarrowThreads)
   if (p.offsets != nullptr) {
     work = false;
     int carry = 0;
-    for (int e0 = 0; e0 < p.experts && !work; e0 += 32) {
+    // one tile, of the last tokens, looks at all experts: where every tile has found its own, nobody else does
+    const bool checks = tile == p.token_tiles - 1;
+    for (int e0 = 0; e0 < p.experts && (!work || checks); e0 += 32) {
       I8Segment s{0, 0, false};
       if (e0 + lane < p.experts) s = i8_segment(p, e0 + lane);
       if (s.bad && warp_idx == 0) ptx::report_status(p.status, kStatusBadArgument, 3, e0 + lane, s.lo);

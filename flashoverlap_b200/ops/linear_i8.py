@@ -21,7 +21,8 @@ def linear_i8(impl, x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
               offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``quantize_rows(x)`` times 8-bit weights, in ``x``'s type: ``y[m, n] = scale[m] * weight_scale[n] * sum_k q[m, k] weight[n, k]``.
 
-    ``impl`` is a single-rank ``OverlapImpl`` (its ``check_status()`` raises if a kernel gave up a wait); ``x`` is [..., K]
+    ``impl`` is a single-rank ``OverlapImpl`` (its ``check_status()`` raises if a kernel gave up a wait or found offsets that are
+    out of order or of range, whose rows it leaves unwritten); ``x`` is [..., K]
     in bf16 or fp16, ``weight`` int8 [N, K], ``weight_scale`` fp32 [N], K a multiple of 16 up to 32768, N of 8.  With
     ``offsets`` (``ExpertOrder.offsets``) ``weight`` is [experts, N, K] and ``weight_scale`` [experts, N]: rows
     ``offsets[e]`` to ``offsets[e + 1] - 1`` of ``x`` [rows, K] are multiplied by ``weight[e]``, other rows of the result are zero.

@@ -186,6 +186,24 @@ def test_offsets_that_are_none(cuda, impl, M, experts):
     assert (c[:4] == 0).all() and (c[-3:] == 0).all() and _close(c[4:10], _ref(a[4:10], b[0], sa[4:10], sb[0]), torch.bfloat16)
 
 
+@pytest.mark.parametrize("M,experts,at", [(1, 40, 33), (2, 40, 39), (2, 1000, 999), (15, 200, 100), (40, 100, 99), (2000, 100, 99)])
+def test_offsets_that_are_none_behind_all_rows(cuda, impl, M, experts, at):
+    """Every row has its expert before the offset that is out of range: that is reported all the same, and the rows are right."""
+    a, b, sa, sb = _operands(cuda, M, 64, 64, experts)
+    offsets = torch.arange(experts + 1, dtype=torch.int32, device=cuda).clamp(max=M)
+    offsets[min(32, experts):] = M
+    c = torch.empty(M, 64, device=cuda, dtype=torch.bfloat16)
+    impl.gemm_i8(a, b, sa, sb, c, offsets)
+    impl.check_status()
+    right = c.clone()
+    offsets[at] = M + 5
+    impl.gemm_i8(a, b, sa, sb, c, offsets)
+    with pytest.raises(RuntimeError, match="bad argument"):
+        impl.check_status()
+    impl.reset_status()
+    assert torch.equal(c, right)
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("shape,N", [((1, 64), 64), ((2, 3, 512), 136), ((512,), 64), ((300, 272), 264)])
 def test_linear(cuda, impl, dt, shape, N):
