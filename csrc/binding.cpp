@@ -171,7 +171,8 @@ bool records(const T&... t) {
 template <typename... T>
 void check_no_gradient(const char* what, const T&... t) {
   check_no_tangent(t...);
-  FO_CHECK(!at::GradMode::is_enabled() || !(t.requires_grad() || ...), what, " has no gradient: call it under no_grad, or detach its inputs");
+  FO_CHECK(!at::GradMode::is_enabled() || !((t.defined() && t.requires_grad()) || ...), what,
+           " has no gradient: call it under no_grad, or detach its inputs");
 }
 
 // Gradients whose own derivatives do not exist: with a graph being recorded for them, differentiating it raises.
@@ -279,6 +280,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm_a
                    "rmsnorm_add_rmsnorm_backward");
   }
   return {DX, DT, DPW, DW, DG};
+}
+
+// As an operator of its own the backward pass has no derivative, and says so.  (On torch's tape `once` does.)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm_add_rmsnorm_backward_op(
+    c10::optional<at::Tensor> GH, c10::optional<at::Tensor> GY, at::Tensor X, at::Tensor T, at::Tensor PW, at::Tensor W,
+    c10::optional<at::Tensor> G, at::Tensor stats, double alpha) {
+  check_no_gradient("rmsnorm_add_rmsnorm_backward", or_undefined(GH), or_undefined(GY), X, T, PW, W, or_undefined(G), stats);
+  return rmsnorm_add_rmsnorm_backward(GH, GY, X, T, PW, W, G, stats, alpha);
 }
 
 struct NormBlockFunction : public torch::autograd::Function<NormBlockFunction> {
@@ -447,6 +456,14 @@ std::tuple<at::Tensor, at::Tensor> moe_combine_backward(at::Tensor GO, c10::opti
                    "moe_combine_backward");
   }
   return {DR, DW};
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_combine_backward_op(at::Tensor GO, c10::optional<at::Tensor> R,
+                                                           c10::optional<at::Tensor> weights, at::Tensor slot,
+                                                           at::Tensor offsets, bool for_rows, bool for_weights,
+                                                           c10::optional<at::Tensor> source) {
+  check_no_gradient("moe_combine_backward", GO, or_undefined(R), or_undefined(weights));
+  return moe_combine_backward(GO, R, weights, slot, offsets, for_rows, for_weights, source);
 }
 
 struct DispatchFunction : public torch::autograd::Function<DispatchFunction> {
@@ -686,14 +703,14 @@ TORCH_LIBRARY(flashoverlap_op, m) {
   m.def("rope_", &rope_);
   m.def("swiglu", &swiglu);
   m.def("rmsnorm_add_rmsnorm", &rmsnorm_add_rmsnorm);
-  m.def("rmsnorm_add_rmsnorm_backward", &rmsnorm_add_rmsnorm_backward);
+  m.def("rmsnorm_add_rmsnorm_backward", &rmsnorm_add_rmsnorm_backward_op);
   m.def("moe_sort(Tensor ids, int experts, int most_ctas=16) -> (Tensor, Tensor, Tensor)", &moe_sort);
   m.def("moe_sort_ctas", [](int64_t choices, int64_t most) { return static_cast<int64_t>(fo::moe_sort_ctas(choices, static_cast<int>(most))); });
   // (source: of the sort; without it the call finds out by itself which rows no slot names, with a launch more)
   m.def("moe_dispatch(Tensor X, Tensor slot, Tensor offsets, Tensor? source=None) -> Tensor", &moe_dispatch);
   m.def("moe_combine(Tensor R, Tensor? weights, Tensor slot, Tensor offsets, Tensor? source=None) -> Tensor", &moe_combine);
   m.def("moe_combine_backward(Tensor GO, Tensor? R, Tensor? weights, Tensor slot, Tensor offsets, bool for_rows, bool for_weights, "
-        "Tensor? source=None) -> (Tensor, Tensor)", &moe_combine_backward);
+        "Tensor? source=None) -> (Tensor, Tensor)", &moe_combine_backward_op);
   m.def("quantize_rows", &quantize_rows);
   m.def("reorder", &reorder);
   m.def("unreorder", &unreorder);

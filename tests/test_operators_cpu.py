@@ -35,3 +35,22 @@ def test_sorts_where_large_clusters_have_no_place(lib):
         for choices in (0, 1, 2048, 2049, 8192, 8193, 2 ** 31 - 1):
             wanted = 1 if choices <= 2048 else 8 if choices <= 8192 else 16
             assert ctas(choices, most) == max(c for c in (1, 8, 16) if c <= min(most, wanted))
+
+
+def test_backward_passes_as_operators_have_no_gradient_to_lose(lib):
+    op = torch.ops.flashoverlap_op
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(64, dtype=torch.bfloat16)
+    order = (torch.zeros(4, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    y, p, stats = torch.zeros(8, 64, dtype=torch.bfloat16), torch.ones(4, 2), torch.zeros(4, 2)
+    for grad in (x, y, p):
+        grad.requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            op.moe_combine_backward(x, y, p, *order, True, True)
+        grad.requires_grad_(False)
+    for grad in (x, w, stats):
+        grad.requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            op.rmsnorm_add_rmsnorm_backward(x, None, x, x, w, w, None, stats, 1.0)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):
+            op.rmsnorm_add_rmsnorm_backward(x, None, x, x, w, w, None, stats, 1.0)
+        grad.requires_grad_(False)
