@@ -133,9 +133,12 @@ cudaError_t dispatch(const GemmI8Plan& plan, const GemmI8Maps& maps, const GemmI
 // 256 x 28672 x 8192: 47 and 80; 192 x 1024 x 8192: 14 and 6; 4096 rows of 64 experts x 3584 x 4096: 162 and 188, 512 rows: 137 and 125.
 namespace {
 
-constexpr int kPairs = 74;
+constexpr int kPairs = 74;  // of a whole B200; where fewer SMs are seen the choice is for more of them, the launch asks the device
 
 // Weight matrices that are used, and the tiles of `rows` tokens that each has: about half of a tile is empty at an expert's end.
+// The counts are on the device, so every expert is taken to have its share.  Shares that fall with the expert's rank to the power of 1.5
+// cost little (64 experts x 3584 x 4096, chosen and best: 256 rows 92 and 91 us, 512 rows 117 and 115, 4096 rows 249 and 227), all rows
+// for one expert more (256 rows 29 and 10 us, 512 rows 41 and 11, 4096 rows 46 and 45).
 struct I8Load {
   double matrices, tiles_each;
 };
@@ -145,9 +148,12 @@ I8Load i8_load(int M, int experts, bool grouped, int rows) {
   return I8Load{used, std::max(1.0, M / used / rows + 0.5)};
 }
 
-// mt: 1, or 2 for tiles of 512 x 256.  Those take 0.66 us a k-block where the call is bound by power, and that is what they are for:
-// under sustained load 8192 x 8192 x 28672 takes 1303 us in them and 1365 in tiles of 256, but 8192 x 28672 x 8192 1378 and 1340,
-// 16384 x 8192 x 3584 368 and 352, 4096 x 4096 x 4096 55 and 50.
+// mt: 1, or 2 for tiles of 512 x 256.  Those save power, which is what binds sustained calls, but nothing hides their epilogue, so they want
+// a long K, and whole waves of their larger tiles.  Sustained, tiles of 256 and of 512 rows, us: 8192 x 8192 x 8192 377, 384; x 12288 568, 566;
+// x 16384 763, 747; x 20480 959, 928; x 28672 1342, 1288; 1024 x 8192 x 28672 187, 176; but 8192 x 28672 x 8192 1340, 1378; 4096 x
+// 8192 x 28672 (3.5 waves of large tiles) 675, 690; 8192 x 5120 x 17920 535, 547.  0.66 us a k-block is their rate under load and 0.34 the
+// other tiles' by themselves (0.42 under load), so that the model takes tall tiles only where their waves are well filled: it does in the cases
+// above from 20480 on that they win, leaves 2 % at 16384 and 4 % of 2048 x 8192 x 28672 (357, 344), and takes them in none that they lose.
 constexpr int kTallTilesK = 16384;
 
 double wide_time(int M, int N, int K, int experts, bool grouped, int mt = 1) {

@@ -4,11 +4,11 @@
 // operand ring holds the same 128 bytes of every row as there, which are 128 elements of K instead of 64, and one
 // tcgen05.mma.kind::i8 takes 32 of them in the time kind::f16 takes 16.  The accumulators are exact 32-bit integers; the
 // epilogue converts each once, multiplies by the two scales in fp32 and rounds to 16 bits.  Bound by the tensor pipe (94-96 % of its
-// cycles) and, under load, by power: 8192^3 298 us (3.7 PFLOP/s) cold, 384 us (2.9) sustained.
+// cycles) and, under load, by power: 8192^3 298 to 320 us (3.7 to 3.4 PFLOP/s) by itself, 378 us (2.9) sustained.
 //
 // Narrow: a batch of few tokens is bound by the weights' way through HBM, so here the weights are the 128 rows of the
 // MMA and the tokens its 16 to 128 columns: no tensor-core row is spent on tokens that are not there, and a k-block
-// costs the weights' 16 KB and little else (1 x 28672 x 8192: 38 us, 6.2 TB/s, against 55 us wide).  The CTAs of a cluster share a tile by splitting K and add their partial sums,
+// costs the weights' 16 KB and little else (1 x 28672 x 8192: 39 us, 6.0 TB/s, against 55 us wide).  The CTAs of a cluster share a tile by splitting K and add their partial sums,
 // exact integers, through distributed shared memory.
 //
 // Rows by expert.  The wide kernel's units are 256-row tiles that start at each expert's first row; the number

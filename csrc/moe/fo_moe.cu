@@ -37,8 +37,9 @@ __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr)
 // expert in a row of its own in shared memory; the counts of the warps and, through distributed shared memory, of the CTAs in
 // front of it give each warp its first row for every expert, and a second walk over the same run hands the rows out, 32
 // choices a step: ballots over the expert's bits tell each lane which others have its expert (half the time of match.any, whose
-// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us with eight CTAs).  Bound by latency:
-// 16 x 8 choices 5.2 us, 8192 x 8 of 64 9.6 us, 16384 x 8 of 256 14 us.
+// cost goes with the number of different experts: 16384 x 8 of 256 in 25 against 41 us with eight CTAs).  Bound by latency; back to
+// back in a graph, and in brackets cold under a profiler: 16 x 8 choices 2.5 us (6.2), 8192 x 8 of 64 7.0 us (11.8), 16384 x 8 of
+// 256 11.5 us (16.1).
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     moe_sort_kernel(const Id* __restrict__ ids, int64_t n, int experts, int32_t* __restrict__ slot,
@@ -258,7 +259,8 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // Bound by the rows written: every token's row is read once.  A thread copies one vector of a token to its top_k rows.
-// 8192 x 8 rows of 4096: 97 us (6.2 TB/s), 16384 x 2 of 8192: 124 us (6.5 TB/s).
+// 8192 x 8 rows of 4096: 97 us (6.2 TB/s), 16384 x 2 of 8192: 129 us (6.2 TB/s).  32 registers, for eight CTAs an SM: rows that
+// are zeros wait for nothing but warps (8192 x 4 rows of 4096, a quarter with a choice, with its sort 59.0 us, at 48 registers 63).
 __global__ void __launch_bounds__(kRowThreads, 8)
     moe_dispatch_kernel(const uint4* __restrict__ X, const int32_t* __restrict__ slot,
                         const int32_t* __restrict__ offsets, NamedRows named, uint4* __restrict__ R,
@@ -304,8 +306,8 @@ __device__ __forceinline__ void unpack8(const uint4& p, float2 (&f)[4]) {
 }
 
 // Bound by the rows read.  A thread sums VPT vectors of a token over its top_k rows, in their order; KC rows of them are in flight at
-// once, and where a token has few rows more of its vectors are (one vector a thread: 16384 x 2 rows of 8192 in 316 us, now 130;
-// 8192 x 8 of 4096: 93 us, 6.5 TB/s).
+// once, and where a token has few rows more of its vectors are (one vector a thread: 16384 x 2 rows of 8192 in 316 us, now 131;
+// 8192 x 8 of 4096: 94 us, 6.4 TB/s).
 template <bool BF16, int KC, int VPT>
 __global__ void __launch_bounds__(kRowThreads)
     moe_combine_kernel(const uint4* __restrict__ R, const void* __restrict__ w, bool f32,
@@ -365,8 +367,8 @@ __global__ void __launch_bounds__(kRowThreads)
 }
 
 // Bound by memory: the token's gradient is read once, every row of the experts is read (for its weight's gradient) and its
-// gradient written.  A CTA takes a token, three of them an SM; the dots are summed over its threads in a fixed order.  8192 x 8 rows of 4096: 183 us
-// (6.2 TB/s; 194 with two an SM), 16384 x 2 of 8192: 215 us (6.2 TB/s).
+// gradient written.  A CTA takes a token, three of them an SM; the dots are summed over its threads in a fixed order.  8192 x 8 rows
+// of 4096: 182 us (6.3 TB/s; 194 with two an SM), 16384 x 2 of 8192: 212 us (6.3 TB/s).
 template <bool BF16, int KC, int VPT, bool ROWS, bool WEIGHTS>
 __global__ void __launch_bounds__(kRowThreads, 3)
     moe_combine_backward_kernel(const uint4* __restrict__ GO, const uint4* __restrict__ R, const void* __restrict__ w,

@@ -154,8 +154,8 @@ __device__ __forceinline__ int owner_of_row(int row, int of, int rows) {
 
 // Bound by memory: 8 bytes an element.  A CTA takes a run of rows; a thread owns VPT vectors of a row, and what it needs of the
 // weights and of the gate's line stays in its registers: beside the ring there is little L1, and rows that fetched them again
-// from the L2 waited for them (8192 x 4096: 57 -> 47 us, 16384 x 1024: 33 -> 27 us, cold; 16384 x 8192: 183 us either way,
-// 5.9 TB/s).  Rows of one vector a thread leave registers for two sets of CTAs.
+// from the L2 waited for them (8192 x 4096: 57 -> 48 us; 16384 x 1024, cold: 33 -> 27 us; 16384 x 8192 no difference: 177 us,
+// 6.1 TB/s).  Rows of one vector a thread leave registers for two sets of CTAs.
 template <bool BF16, int VPT, int CTAS, int GATE>
 __global__ void __launch_bounds__(kMaxThreads, 1)
     norm_block_kernel(const uint16_t* __restrict__ X, const uint16_t* __restrict__ T, const uint16_t* __restrict__ PW,
@@ -329,9 +329,9 @@ struct BackwardArgs {
 // n1 = T r1, n2 = H r2:  dH = GH + r2 (GY W - n2 mean(GY W n2)),  dX = alpha dH,  b = dH G PW,
 // dT = r1 (b - n1 mean(b n1)),  dW = sum GY n2,  and with m = dH n1 summed over the rows of a line of the gate,
 // dG = PW sum m,  dPW = sum over the lines of G sum m: one column sum a row serves both.
-// 12 bytes an element: 8192 x 8192 145 us (5.5 TB/s), 16384 x 8192 without a gate 270 us (6.0 TB/s).  Bound by memory, and by the
+// 12 bytes an element: 8192 x 8192 145 us (5.5 TB/s), 16384 x 8192 without a gate 271 us with the sums (5.9 TB/s).  Bound by memory, and by the
 // latencies of 16 warps an SM, all that the column sums' registers leave.  Column sums stay in registers over a CTA's rows and are
-// added up over the CTAs by the two kernels below, in a fixed order (6 us).
+// added up over the CTAs by the two kernels below, in a fixed order (6 us behind this kernel; 11 us cold, by itself under a profiler).
 template <bool BF16, int VPT, int CTAS, int GATE>
 __global__ void __launch_bounds__(kMaxThreads, 1) norm_block_backward_kernel(const __grid_constant__ BackwardArgs p) {
   extern __shared__ uint4 ring_words[];

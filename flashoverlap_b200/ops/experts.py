@@ -1,8 +1,9 @@
 """Rows sorted by expert and back, with gradients: what stands around the products of a mixture-of-experts block.
 
-``moe_sort`` turns the router's choices into an order, ``moe_dispatch`` brings the tokens' rows into it (the form
-``OverlapImpl.gemm_all2all`` and the products by expert take), ``moe_combine`` sums the experts' rows back
-into their tokens with the router's weights.
+``moe_sort`` turns the router's choices into an order, ``moe_dispatch`` brings the tokens' rows into it (the form the
+products by expert take; where a rank's experts follow one another it is also sorted by rank, as ``OverlapImpl.gemm_all2all``
+takes its rows, which leaves out the rank's own), ``moe_combine`` sums the experts' rows back into their tokens with the
+router's weights.
 """
 from __future__ import annotations
 

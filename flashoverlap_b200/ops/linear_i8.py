@@ -10,7 +10,8 @@ from ._native import native
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of ``x`` [rows, dim] in bf16 or fp16: with ``a = max(max|x[r]|, 2^-100)``, ``scale[r] = a / 127`` and
-    ``q[r]`` the int8 nearest to ``x[r] * (127 / a)``, ties to even, every operation rounded in fp32.
+    ``q[r]`` the int8 nearest to ``x[r] * (127 / a)``, ties to even, every operation rounded in fp32.  (The quotient is one division;
+    torch's ``127.0 / a`` on a GPU is a reciprocal and a product, another number for a quarter of the rows.)
 
     ``dim`` is a multiple of 8 up to 32768.  A row with a NaN or an infinity gets zeros and the scale NaN, so that
     what is computed from it is NaN."""
