@@ -8,8 +8,8 @@
 //
 // Narrow: a batch of few tokens is bound by the weights' way through HBM, so here the weights are the 128 rows of the
 // MMA and the tokens its 16 to 128 columns: no tensor-core row is spent on tokens that are not there, and a k-block
-// costs the weights' 16 KB and little else (1 x 28672 x 8192: 39 us, 6.0 TB/s, against 55 us wide).  The CTAs of a cluster share a tile by splitting K and add their partial sums,
-// exact integers, through distributed shared memory.
+// costs the weights' 16 KB and little else (1 x 28672 x 8192: 39 us, 6.0 TB/s, against 55 us wide).  The CTAs of a cluster share
+// a tile by splitting K and add their partial sums, exact integers, through distributed shared memory.
 //
 // Rows by expert.  The wide kernel's units are 256-row tiles that start at each expert's first row; the number
 // of units is only known on the device, so every CTA sums up the experts' tiles in its prologue and finds a unit's

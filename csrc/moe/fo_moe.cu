@@ -194,9 +194,9 @@ __device__ __forceinline__ void zero_rows(uint4* rows, int64_t first, int64_t la
 // after a row, which is named if the choice that back[row] holds names it; so are all rows of a sorted order with its own
 // sources.  Where it does not, nobody names the row if `back` is the scratch of moe_inverse_kernel (`exact`), but sources may
 // also be of something else: then the CTA goes through all slots.  8192 x 8 rows of 512: 13.0 us sorted (12.8 without any of this),
-// 33 with a tenth dropped; with a scratch 14.3 and 14.6, but one launch more also for the host, which waits for 16 x 8 rows (13.8 us a
-// sort and dispatch either way).  So the scratch is made where a call brings no sources, and for more than kNamedScan choices,
-// since the search's cost grows with their square (8192 x 8 rows of 4096: 96, 106 with a tenth dropped, and 98 with a scratch).
+// 33 with a tenth dropped; with a scratch 14.3 and 14.6, but one launch more, which small calls pay for on the host.  So the scratch is
+// made where a call brings no sources, and for more than kNamedScan choices, since the search's cost grows with their square
+// (8192 x 8 rows of 4096: 96 us, 106 with a tenth dropped, and 98 with a scratch).
 constexpr int64_t kNamedScan = 65536;
 
 struct NamedRows {

@@ -325,6 +325,39 @@ def test_replayed_graph_and_another_stream(cuda):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("tokens", [300, 9000])
+def test_choices_dropped_between_replays(cuda, tokens):
+    """Two graphs of an order whose slots are edited in place, replayed on two streams at once: every replay goes by the slots as they are."""
+    dt, top_k, dim = torch.bfloat16, 8, 128
+    order, x, y, w = _problem(cuda, dt, tokens, top_k, 16, dim)
+    order = order._replace(slot=order.slot.clone())
+    go = torch.randn(tokens, dim, device=cuda).to(dt)
+
+    def step(source):
+        return (torch.ops.flashoverlap_op.moe_dispatch(x, order.slot, order.offsets, source),
+                *torch.ops.flashoverlap_op.moe_combine_backward(go, y, w, order.slot, order.offsets, True, True, source))
+
+    graphs = []
+    for source in (order.source, None):
+        step(source)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(source)
+        graphs.append((graph, out, torch.cuda.Stream()))
+    for _ in range(3):
+        order.slot[torch.rand(order.slot.shape, device=cuda) < 0.2] = -1
+        torch.cuda.synchronize()
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        rows = _rows_ref(x[:, None].expand(-1, top_k, -1), order, tokens * top_k)
+        grad = _rows_ref((go.float()[:, None] * w[..., None]).to(dt), order, tokens * top_k)
+        for _, (r, dr, dw), _ in graphs:
+            assert torch.equal(r, rows) and torch.equal(dr, grad) and (dw[order.slot < 0] == 0).all()
+
+
 def test_refuses(cuda):
     order, x, y, w = _problem(cuda, torch.bfloat16, 20, 2, 4, 64)
     ids = torch.zeros(20, 2, dtype=torch.int32, device=cuda)
